@@ -38,6 +38,9 @@ extern "C" {
 /* Activation-quantisation modes (flags of ltxfp8_quantize_1x128). */
 #define LTXFP8_QUANT_TORCH 0  /* s = (1/amax)*448, IEEE roundings: bit-exact with blockwise_quantize_torch */
 #define LTXFP8_QUANT_TRITON 1 /* s = 448/amax, 1/s via div.full.f32: the arithmetic of the Triton kernel */
+#define LTXFP8_QUANT_FINITE 2 /* scale = max(amax, 448 * 2^-126) / 448, code = e4m3(x / scale), within 1 ulp: an all-zero
+                                 group gets zero codes (the modes above give NaN there).  ltxfp8_quantize_1x128 only;
+                                 the residual-path operators at the end of this file always quantise this way */
 
 /* Input dtypes for ltxfp8_quantize_weight_128x128. */
 #define LTXFP8_DTYPE_F32 0
@@ -55,7 +58,7 @@ const char* ltxfp8_last_error(void);
  *   x      bf16 [M, K], row stride x_ld elements (x_ld >= K, x_ld % 8 == 0)
  *   q      e4m3 [M, K], row stride q_ld bytes (q_ld % 8 == 0)
  *   sfa    fp32, element (m, kb) at sfa[kb * sfa_ld + m], sfa_ld >= M
- *   K % 128 == 0.  flags: LTXFP8_QUANT_TORCH or LTXFP8_QUANT_TRITON.
+ *   K % 128 == 0.  flags: LTXFP8_QUANT_TORCH, LTXFP8_QUANT_TRITON or LTXFP8_QUANT_FINITE.
  * Replaces the Triton op blockwise::quantize with use_gelu=False
  * (ltx-kernels/src/ltx_kernels/blockwise/triton_ops.py:128-151, kernel :102-126)
  * and blockwise_quantize_torch (functional.py:138-144).
@@ -330,6 +333,92 @@ int ltxfp8_gemm_set_variant(int variant);
  * runtime form of that term.
  */
 int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_t K, int64_t r, void* stream);
+
+/* ------------------------------------------------------------------ residual path and training
+ *
+ * Operators of a pre-norm block around the blockwise-FP8 linears, forward and backward.
+ * No reference counterpart (the reference's blockwise path has no gradient, no ungated
+ * residual and no gain in its norms).  Quantised outputs use LTXFP8_QUANT_FINITE and the
+ * layout of ltxfp8_quantize_1x128 with q_ld = the row length.  Row operands are bf16 with
+ * 16-byte aligned rows (row strides in elements, multiples of 8); outputs are contiguous.
+ * All arithmetic is fp32, each output rounded once; sums over tokens are taken in a fixed
+ * order, so results repeat bit for bit on the same device.
+ */
+
+/*
+ * RMS norm with the residual's addition: h = bf16(x + residual) (h = x when residual is
+ * NULL; then h must be NULL), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight;
+ * with q != NULL (q, sfa) = 1x128 quant of y, otherwise out = bf16(y).  h may be x or
+ * residual (in place).  weight [H] of weight_dtype (LTXFP8_DTYPE_F32 or _BF16) or NULL;
+ * rstd fp32 [M] or NULL.  H % 128 == 0, H <= 16384.
+ */
+int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t M,
+                             int64_t H, const void* weight, int weight_dtype, float eps, void* h, void* q, float* sfa,
+                             int64_t sfa_ld, void* out, float* rstd, void* stream);
+
+/*
+ * Its gradient: g = dy * weight, xhat = h * rstd, dx = rstd * (g - xhat * mean(g * xhat))
+ * + dh, dweight = sum over rows of dy * xhat (in weight_dtype).  dh (the gradient that
+ * reaches h along the residual stream) and dweight may be NULL; dx is the gradient of x
+ * and of the residual alike and may be dh or dy when that is contiguous.  dweight needs a
+ * workspace of ltxfp8_rms_norm_backward_workspace_bytes.  M == 0 gives dweight = 0.
+ */
+int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* rstd,
+                             const void* weight, int weight_dtype, const void* dh, int64_t dh_ld, int64_t M, int64_t H,
+                             void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+int ltxfp8_rms_norm_backward_workspace_bytes(int64_t M, int64_t H, size_t* bytes);
+
+/* Activations of the calls below. */
+#define LTXFP8_ACT_NONE 0
+#define LTXFP8_ACT_GELU_TANH 1
+#define LTXFP8_ACT_SILU 2
+
+/*
+ * ltxfp8_gemm with activation and residual in its epilogue, rounded once:
+ *   D = bf16( act( sum_kb sfa[m,kb] sfb[n/128,kb] (A W^T)_kb + bias ) + residual )
+ * residual bf16 [M, N] with row stride residual_ld (a multiple of 8), or NULL; it may be D.
+ * workspace: split-K scratch of ltxfp8_gemm_workspace_bytes, optional as for ltxfp8_gemm.
+ */
+int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const void* W, const float* sfb,
+                         const float* bias, const void* residual, int64_t residual_ld, void* D, int64_t M, int64_t N,
+                         int64_t K, int activation, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Activation with an 8-bit checkpoint of its input: (yq, ys) = 1x128 quant of act(z),
+ * (zq, zs) = 1x128 quant of z.  z bf16 [M, N], N % 128 == 0; LTXFP8_ACT_GELU_TANH or _SILU.
+ */
+int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, int activation, void* yq, float* ys,
+                             int64_t ys_ld, void* zq, float* zs, int64_t zs_ld, void* stream);
+
+/*
+ * Its gradient from the checkpoint: dz = dy * act'(zq * zs), written as bf16 (dz), as
+ * 1x128 codes (dzq, dzs) or both, and dbias fp32 [N] = sum over rows of dz (NULL: not
+ * wanted; it needs a workspace of ltxfp8_act_backward_workspace_bytes).  dz may be dy when
+ * that is contiguous.  M == 0 gives dbias = 0.
+ */
+int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const float* zs, int64_t zs_ld, int64_t M,
+                        int64_t N, int activation, void* dz, void* dzq, float* dzs, int64_t dzs_ld, float* dbias,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes);
+
+/*
+ * Weight gradient: out[n, k] = bf16( alpha * sum over m of g[m, n] * x[m, k] ).
+ * g bf16 [M, N] (N % 16 == 0); x [M, K] (K % 128 == 0) either e4m3 codes with scales xs
+ * (element (m, kb) at xs[kb * xs_ld + m]; x_ld in bytes, a multiple of 16), each value
+ * expanded to bf16, or bf16 when xs is NULL.  transposed: out is [K, N] instead of [N, K].
+ * Needs a workspace of ltxfp8_wgrad_workspace_bytes (0: none).  M == 0 gives zeros.
+ */
+int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const float* xs, int64_t xs_ld, float alpha,
+                 void* out, int transposed, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                 void* stream);
+int ltxfp8_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes);
+
+/*
+ * Transpose of a blockwise-FP8 weight for the input gradient dX = dY W: codes [N, K] ->
+ * qt [K, N], scales [N/128, K/128] -> sfbt [K/128, N/128].  Not in place.
+ */
+int ltxfp8_transpose_weight_128x128(const void* q, const float* sfb, int64_t N, int64_t K, void* qt, float* sfbt,
+                                    void* stream);
 
 /*
  * Read (and optionally clear) the device status word that kernels set when a

@@ -1,0 +1,201 @@
+// An activation function with the 8-bit checkpoint of its input, and its use in the
+// backward pass (streaming kernels, sm_100a).
+//
+//   forward   (yq, ys) = 1x128 quant of act(z)   the next GEMM's operand
+//             (zq, zs) = 1x128 quant of z        all that the backward pass keeps of z
+//   backward  z~ = zq * zs,  dz = dy * act'(z~), as bf16 (weight gradients), as 1x128 codes
+//             (the input-gradient GEMM's operand) and summed over tokens (bias gradient)
+//
+// The activations and their derivatives are in activation.cuh; everything is fp32 and unrounded up to the outputs' own rounding.
+#pragma once
+
+#include "activation.cuh"
+#include "residual_norm.cuh"
+
+namespace ltxfp8 {
+
+// 16 e4m3 codes -> fp32 (exact).
+__device__ __forceinline__ void codes16_to_f2(const uint4& v, float2 (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __half22float2(__half2(
+        __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xFFFFu), __NV_E4M3)));
+    f[2 * i + 1] =
+        __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3)));
+  }
+}
+
+struct ActSaveParams {
+  const __nv_bfloat16* z;
+  int64_t z_ld, M, N;
+  uint32_t groups;  // N / 128
+  uint32_t magic;   // ceil(2^32 / groups): k / groups = umulhi(k, magic) for the k used here
+  uint8_t* yq;
+  float* ys;
+  int64_t ys_ld;
+  uint8_t* zq;
+  float* zs;
+  int64_t zs_ld;
+};
+
+constexpr int kActSaveUnroll = 2;
+constexpr int kActSaveGroups = 32 * kActSaveUnroll;  // 1x128 groups of a 256-thread block
+
+template <int kAct>
+__global__ void __launch_bounds__(256) act_quantize_save_kernel(const ActSaveParams p) {
+  const int64_t g0 = static_cast<int64_t>(blockIdx.x) * kActSaveGroups;
+  const int64_t row0 = g0 / p.groups;
+  const uint32_t kb0 = static_cast<uint32_t>(g0 - row0 * p.groups);
+  const int l8 = threadIdx.x & 7;
+  Run16 v[kActSaveUnroll];
+  int64_t row[kActSaveUnroll];
+  uint32_t kb[kActSaveUnroll];
+#pragma unroll
+  for (int u = 0; u < kActSaveUnroll; ++u) {
+    const uint32_t k = kb0 + (threadIdx.x >> 3) + 32u * u;
+    const uint32_t dr = p.groups == 1 ? k : __umulhi(k, p.magic);
+    row[u] = row0 + dr;
+    kb[u] = k - dr * p.groups;
+    v[u] = row[u] < p.M ? ld_run(p.z + row[u] * p.z_ld + kb[u] * 128 + l8 * kRunLen) : zero_run();
+  }
+#pragma unroll
+  for (int u = 0; u < kActSaveUnroll; ++u) {
+    float2 z[8], y[8];
+    run_to_f2(v[u], z);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = act_apply<kAct>(z[j]);
+    float zi, yi;
+    const uint4 zc = quant_run16(z, zi);
+    const uint4 yc = quant_run16(y, yi);
+    if (row[u] < p.M) {
+      const int64_t off = row[u] * p.N + kb[u] * 128 + l8 * kRunLen;
+      *reinterpret_cast<uint4*>(p.yq + off) = yc;
+      *reinterpret_cast<uint4*>(p.zq + off) = zc;
+      if (l8 == 0) {
+        p.ys[static_cast<int64_t>(kb[u]) * p.ys_ld + row[u]] = yi;
+        p.zs[static_cast<int64_t>(kb[u]) * p.zs_ld + row[u]] = zi;
+      }
+    }
+  }
+}
+
+struct ActBwdParams {
+  const __nv_bfloat16* dy;
+  int64_t dy_ld, M, N;
+  const uint8_t* zq;
+  const float* zs;
+  int64_t zs_ld;
+  int groups;         // N / 128
+  __nv_bfloat16* dz;  // [M, N] or null
+  uint8_t* dzq;       // [M, N] or null
+  float* dzs;
+  int64_t dzs_ld;
+  float* db_part;  // [gridDim.y, N] partial column sums, or null
+};
+
+// A block owns kG adjacent 1x128 groups (8 lanes each) and walks the rows with stride
+// gridDim.y * rows-per-pass, so the bias gradient of its columns stays in registers; the
+// partial sums of the gridDim.y row shares are added by col_sum_kernel in a fixed order.
+constexpr int kActBwdUnroll = 2;
+
+template <int kAct, int kG>
+__global__ void __launch_bounds__(256) act_backward_kernel(const ActBwdParams p) {
+  constexpr int kRows = 32 / kG;  // rows of one pass
+  __shared__ float db_rows[kRows][kG * 128];
+  const int t = threadIdx.x % (8 * kG), r = threadIdx.x / (8 * kG);
+  const int kb = blockIdx.x * kG + t / 8;
+  const bool col_ok = kb < p.groups;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kG * 128 + t * kRunLen;
+  float2 db[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) db[j] = make_float2(0.0f, 0.0f);
+
+  for (int64_t m0 = static_cast<int64_t>(blockIdx.y) * (kRows * kActBwdUnroll); m0 < p.M;
+       m0 += static_cast<int64_t>(gridDim.y) * (kRows * kActBwdUnroll)) {
+    Run16 vy[kActBwdUnroll];
+    uint4 vz[kActBwdUnroll];
+    float sc[kActBwdUnroll];
+#pragma unroll
+    for (int u = 0; u < kActBwdUnroll; ++u) {
+      const int64_t m = m0 + u * kRows + r;
+      const bool ok = col_ok && m < p.M;
+      vy[u] = ok ? ld_run(p.dy + m * p.dy_ld + col) : zero_run();
+      vz[u] = ok ? *reinterpret_cast<const uint4*>(p.zq + m * p.N + col) : make_uint4(0, 0, 0, 0);
+      sc[u] = ok ? __ldg(p.zs + static_cast<int64_t>(kb) * p.zs_ld + m) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kActBwdUnroll; ++u) {
+      const int64_t m = m0 + u * kRows + r;
+      const bool ok = col_ok && m < p.M;
+      float2 d[8], z[8];
+      run_to_f2(vy[u], d);
+      codes16_to_f2(vz[u], z);
+      const float2 s2 = make_float2(sc[u], sc[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        d[j] = __fmul2_rn(d[j], act_grad<kAct>(__fmul2_rn(z[j], s2)));
+        db[j] = __fadd2_rn(db[j], d[j]);
+      }
+      if (p.dz != nullptr && ok) st_run(p.dz + m * p.N + col, f2_to_run(d));
+      if (p.dzq != nullptr) {
+        float inv;
+        const uint4 c = quant_run16(d, inv);
+        if (ok) {
+          *reinterpret_cast<uint4*>(p.dzq + m * p.N + col) = c;
+          if ((t & 7) == 0) p.dzs[static_cast<int64_t>(kb) * p.dzs_ld + m] = inv;
+        }
+      }
+    }
+  }
+  if (p.db_part == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) *reinterpret_cast<float2*>(&db_rows[r][t * kRunLen + 2 * j]) = db[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < kG * 128; c += 256) {
+    float s = db_rows[0][c];
+#pragma unroll
+    for (int i = 1; i < kRows; ++i) s += db_rows[i][c];
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * kG * 128 + c;
+    if (n < p.N) p.db_part[static_cast<int64_t>(blockIdx.y) * p.N + n] = s;
+  }
+}
+
+// Transpose of a blockwise-FP8 weight: codes [N, K] -> [K, N], scales [N/128, K/128] ->
+// [K/128, N/128], one 128 x 128 block per thread block: the operand of the input-gradient
+// GEMM dX = dY W.  Codes pass through a padded shared tile in 4 x 4 byte squares.
+__global__ void __launch_bounds__(256) transpose_weight_kernel(const uint8_t* __restrict__ q,
+                                                               const float* __restrict__ s, int64_t N, int64_t K,
+                                                               uint8_t* __restrict__ qt, float* __restrict__ st) {
+  __shared__ uint32_t tile[128][33];  // row n, four codes a word
+  const int64_t kb = blockIdx.x, nb = blockIdx.y;
+  const uint8_t* src = q + nb * 128 * K + kb * 128;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 32 + (threadIdx.x >> 3), c = threadIdx.x & 7;
+    const uint4 v = *reinterpret_cast<const uint4*>(src + row * K + c * 16);
+    tile[row][c * 4] = v.x;
+    tile[row][c * 4 + 1] = v.y;
+    tile[row][c * 4 + 2] = v.z;
+    tile[row][c * 4 + 3] = v.w;
+  }
+  __syncthreads();
+  uint8_t* dst = qt + kb * 128 * N + nb * 128;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // square (n4, k4): rows n4*4 .. +3 of word k4 -> rows k4*4 .. +3, word n4
+    const int n4 = threadIdx.x & 31, k4 = i * 8 + (threadIdx.x >> 5);
+    const uint32_t a = tile[n4 * 4][k4], b = tile[n4 * 4 + 1][k4], c = tile[n4 * 4 + 2][k4], d = tile[n4 * 4 + 3][k4];
+    const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+    const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+    uint32_t* o = reinterpret_cast<uint32_t*>(dst + static_cast<int64_t>(k4) * 4 * N) + n4;
+    const int64_t ld = N / 4;
+    o[0] = __byte_perm(ab0, cd0, 0x5410);
+    o[ld] = __byte_perm(ab0, cd0, 0x7632);
+    o[2 * ld] = __byte_perm(ab1, cd1, 0x5410);
+    o[3 * ld] = __byte_perm(ab1, cd1, 0x7632);
+  }
+  if (threadIdx.x == 0) st[kb * (N / 128) + nb] = s[nb * (K / 128) + kb];
+}
+
+}  // namespace ltxfp8

@@ -28,10 +28,14 @@
 //               its 1x128 requantisation to e4m3 for the next layer (codes
 //               written over the consumed bf16, then stored by TMA), so that
 //               work overlaps the next tile's K loop.
+//   residual    with kAct >= 0 the epilogue is instead bf16(act(acc + bias) + residual), one
+//               rounding: the store warps TMA-load the residual tile into the staging tile
+//               while the K loop runs, the promotion warps read it there, add and write back.
 //   LoRA        alpha * (x A^T) B^T is folded in as extra K blocks of bf16 MMAs
 //               (kind::f16) over [x A^T | B], promoted with scale alpha.
 #pragma once
 
+#include "activation.cuh"
 #include "gelu.cuh"
 #include "ptx.cuh"
 
@@ -73,6 +77,7 @@ enum GemmFlags : int {
   kGemmRequantTriton = 16,  // requantisation scales as the Triton quantiser computes them (div.full)
   kGemmWeightFp6 = 32,      // W is e2m3 codes packed 6 bits each in the tensor core's order
                             // (ltxfp8_fp6_to_tc), its scales already multiplied by 2^-6
+  kGemmResidual = 64,       // kAct >= 0: add the bf16 residual after the activation
 };
 
 // Scale pair of a requantised 1x128 group from its abs-max: the Triton quantiser's
@@ -96,6 +101,7 @@ enum GemmStatus : unsigned int {
   kStDrain = 0x47010005u,
   kStStagingFull = 0x47010006u,
   kStStagingEmpty = 0x47010007u,
+  kStResidual = 0x47010008u,
 };
 
 struct GemmParams {
@@ -121,6 +127,8 @@ struct GemmParams {
   int k_splits;
   int kb_per_split;
   float* ws;
+  const __nv_bfloat16* res;  // residual [M, N], row stride res_ld (kGemmResidual)
+  int64_t res_ld;
 };
 
 // Grouped rasterisation: consecutive tile indices walk group_m M-tiles down a
@@ -224,7 +232,17 @@ __device__ __forceinline__ bool promote_kblock(uint64_t* tfull, uint64_t* tempty
   return true;
 }
 
-template <bool kGelu, bool kRequant>
+// bf16 of a column pair through the residual epilogue: act(z) + r, one rounding.
+template <int kAct>
+__device__ __forceinline__ uint32_t residual_pair(float2 acc, float2 bias, uint32_t res) {
+  float2 y = act_apply<kAct>(__fadd2_rn(acc, bias));
+  y = __fadd2_rn(y, make_float2(__uint_as_float(res << 16), __uint_as_float(res & 0xFFFF0000u)));
+  return pack_bf16x2(y.x, y.y);
+}
+
+// kAct < 0: the reference's chain of roundings (kGelu, kRequant).  kAct >= 0 (an ActKind,
+// with kGelu = kRequant = false): the residual epilogue, with tmQ the residual's map.
+template <bool kGelu, bool kRequant, int kAct = -1>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     fp8_blockwise_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                               const __grid_constant__ CUtensorMap tmLX, const __grid_constant__ CUtensorMap tmLB,
@@ -242,7 +260,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint64_t* stg_full = tempty + 2;     // [1] promotion warps -> store warps
   uint64_t* stg_empty = stg_full + 1;  // [1] store warps -> promotion warps
   uint64_t* drain = stg_empty + 1;     // [1]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* res_full = drain + 1;      // [1] residual tile loaded (kAct >= 0)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 1);
   uint16_t* gelu_tab = reinterpret_cast<uint16_t*>(staging + kStagingBytes + kStagingAmaxBytes + kGemmBarrierBytes);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0);
@@ -261,6 +280,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     mbar_init(stg_full, 8);      // one arrival per promotion warp
     mbar_init(stg_empty, 2);     // one arrival per store warp
     mbar_init(drain, 1);
+    mbar_init(res_full, 2);      // one arrival per store warp
     fence_mbarrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -272,7 +292,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     if (p.k_splits == 1) {
       if (p.flags & kGemmWriteD) tma_prefetch_desc(&tmD);
-      if (kRequant) tma_prefetch_desc(&tmQ);
+      if (kRequant || (kAct >= 0 && (p.flags & kGemmResidual))) tma_prefetch_desc(&tmQ);
     }
   }
   if (warp == 1) {
@@ -371,11 +391,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int pw = warp - 2;
       const bool write_d = (p.flags & kGemmWriteD) != 0;
       uint32_t tcount = 0;
+      const bool has_res = kAct >= 0 && (p.flags & kGemmResidual) != 0;
+      // Lane 0: fetch this warp's slices of tile u's residual into the staging tile (same
+      // boxes and swizzle as the stores).
+      auto load_residual = [&](int u) {
+        int mt, nt;
+        gemm_tile_coords(u, p, mt, nt);
+        const int m0 = mt * kBM, n0 = nt * kBN;
+        uint32_t boxes = 0;
+        for (int h = 0; h < 2; ++h)
+          for (int b4 = 0; b4 < 4; ++b4)
+            boxes += (m0 + h * 64 + pw * 32 < p.M && n0 + b4 * 64 < p.N) ? 1u : 0u;
+        mbar_arrive_expect_tx(res_full, boxes * (32u * 128u));
+        for (int h = 0; h < 2; ++h) {
+          const int rb = h * 64 + pw * 32;
+          for (int b4 = 0; b4 < 4; ++b4)
+            if (m0 + rb < p.M && n0 + b4 * 64 < p.N)
+              tma_load_2d(&tmQ, res_full, staging + b4 * kStagingBlockBytes + rb * 128, n0 + b4 * 64, m0 + rb);
+        }
+      };
+      if constexpr (kAct >= 0) {
+        if (has_res && lane == 0 && static_cast<int>(blockIdx.x) < p.total_tiles) load_residual(blockIdx.x);
+      }
       for (int u = blockIdx.x; u < p.total_tiles; u += gridDim.x, ++tcount) {
         int mt, nt;
         gemm_tile_coords(u, p, mt, nt);
         const int m0 = mt * kBM, n0 = nt * kBN;
-        if (!__all_sync(0xffffffffu, mbar_wait(stg_full, tcount & 1u, kStStagingFull))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(stg_full, tcount & 1u, kStStagingFull))) {
+          if (kAct >= 0 && has_res) mbar_wait(res_full, tcount & 1u, kStDrain);  // the loads in flight land first
+          break;
+        }
         if constexpr (kRequant) {
           // 1x128 requantisation of the staged bf16 values (the reference
           // quantises the bf16 GEMM / GELU output).  One lane per group: step j
@@ -453,6 +498,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // The staging tile may be overwritten once the stores have read it.
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
+        if constexpr (kAct >= 0) {
+          if (has_res && lane == 0 && u + static_cast<int>(gridDim.x) < p.total_tiles) load_residual(u + gridDim.x);
+        }
         if (lane == 0) mbar_arrive(stg_empty);
       }
       if (lane == 0) tma_store_wait_all();
@@ -553,7 +601,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if constexpr (kPost) {
         while (post_c < 16) post_step();  // the previous tile's pass, if the K loop was too short
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(stg_empty, (tcount & 1u) ^ 1u, kStStagingEmpty))) {
+      // (The residual's arrival implies that the previous tile's stores have read theirs.)
+      const bool has_res = kAct >= 0 && (p.flags & kGemmResidual) != 0;
+      if (!__all_sync(0xffffffffu, has_res ? mbar_wait(res_full, tcount & 1u, kStResidual)
+                                           : mbar_wait(stg_empty, (tcount & 1u) ^ 1u, kStStagingEmpty))) {
         ok = false;
         break;
       }
@@ -567,6 +618,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           b1 = __ldg(bias4 + 2 * c + 1);
         }
         const float2 a0 = acc[4 * c], a1 = acc[4 * c + 1], a2 = acc[4 * c + 2], a3 = acc[4 * c + 3];
+        if constexpr (kAct >= 0) {
+          uint4* ptr = reinterpret_cast<uint4*>(staging + gemm_staging_off(r_local, half * 16 + c));
+          const uint4 rv = has_res ? *ptr : make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
+          *ptr = make_uint4(residual_pair<kAct>(a0, make_float2(b0.x, b0.y), rv.x),
+                            residual_pair<kAct>(a1, make_float2(b0.z, b0.w), rv.y),
+                            residual_pair<kAct>(a2, make_float2(b1.x, b1.y), rv.z),
+                            residual_pair<kAct>(a3, make_float2(b1.z, b1.w), rv.w));
+          continue;
+        }
         // The reference applies GELU to the bf16 tensor bf16(acc + bias) and rounds
         // the result to bf16: the second pass reads these values back.
         *reinterpret_cast<uint4*>(staging + gemm_staging_off(r_local, half * 16 + c)) =
@@ -602,7 +662,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // tile's unit partials in split order (deterministic).  One half-warp per (tile
 // row, 128-column group): 16 lanes x 8 columns, so the 1x128 requantisation needs
 // no cross-row reduction.  Epilogue semantics are those of the GEMM kernel.
-template <bool kGelu, bool kRequant>
+template <bool kGelu, bool kRequant, int kAct = -1>
 __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmParams p) {
   const int64_t total = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
@@ -644,6 +704,18 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmParams p) 
     }
   }
   const int64_t off = static_cast<int64_t>(row) * p.N + col;
+  if constexpr (kAct >= 0) {
+    uint4 rv = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
+    if (active && (p.flags & kGemmResidual))
+      rv = *reinterpret_cast<const uint4*>(p.res + static_cast<int64_t>(row) * p.res_ld + col);
+    const float2 z = make_float2(0.0f, 0.0f);  // the bias is in f already
+    if (active)
+      *reinterpret_cast<uint4*>(p.d + off) = make_uint4(residual_pair<kAct>(make_float2(f[0], f[1]), z, rv.x),
+                                                        residual_pair<kAct>(make_float2(f[2], f[3]), z, rv.y),
+                                                        residual_pair<kAct>(make_float2(f[4], f[5]), z, rv.z),
+                                                        residual_pair<kAct>(make_float2(f[6], f[7]), z, rv.w));
+    return;
+  }
   if (active && (p.flags & kGemmWriteD)) {
     *reinterpret_cast<uint4*>(p.d + off) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
                                                       pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));

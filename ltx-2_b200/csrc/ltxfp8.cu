@@ -13,12 +13,15 @@
 #include <mutex>
 #include <string>
 
+#include "act_checkpoint.cuh"
 #include "gemm.cuh"
 #include "gemm_pair.cuh"
 #include "lora.cuh"
 #include "producers.cuh"
 #include "ptx.cuh"
 #include "quant.cuh"
+#include "residual_norm.cuh"
+#include "wgrad.cuh"
 
 using namespace ltxfp8;
 
@@ -86,10 +89,11 @@ struct DeviceInfo {
   bool init = false;
   int sms = 0;
   int major = 0, minor = 0;
-  bool gemm_ready[4] = {false, false, false, false};
+  bool gemm_ready[7] = {};  // by (GELU, requant), then by the residual epilogue's activation
   bool pair_ready[4] = {false, false, false, false};
   int pair_clusters = 0;  // co-resident 2-CTA clusters of the pair kernel
   bool lora_ready = false;
+  bool wgrad_ready[2] = {false, false};  // by x type: bf16, e4m3
   float* static_scratch = nullptr;  // device address of g_gemm_static_scratch (ltxfp8_gemm_static_scratch)
 };
 
@@ -119,12 +123,12 @@ int device_info(DeviceInfo** out) {
   return LTXFP8_OK;
 }
 
-template <bool kGelu, bool kRequant>
+template <bool kGelu, bool kRequant, int kAct = -1>
 int gemm_prepare(DeviceInfo* d) {
-  const int idx = (kGelu ? 1 : 0) | (kRequant ? 2 : 0);
+  const int idx = kAct >= 0 ? 4 + kAct : (kGelu ? 1 : 0) | (kRequant ? 2 : 0);
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (d->gemm_ready[idx]) return LTXFP8_OK;
-  auto kern = fp8_blockwise_gemm_kernel<kGelu, kRequant>;
+  auto kern = fp8_blockwise_gemm_kernel<kGelu, kRequant, kAct>;
   cudaFuncAttributes attr;
   cudaError_t e = cudaFuncGetAttributes(&attr, kern);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(gemm)");
@@ -139,11 +143,11 @@ int gemm_prepare(DeviceInfo* d) {
   return LTXFP8_OK;
 }
 
-template <bool kGelu, bool kRequant>
+template <bool kGelu, bool kRequant, int kAct = -1>
 int gemm_launch(DeviceInfo* d, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& lx,
                 const CUtensorMap& lb, const CUtensorMap& md, const CUtensorMap& mq, const GemmParams& p,
                 cudaStream_t stream) {
-  int rc = gemm_prepare<kGelu, kRequant>(d);
+  int rc = gemm_prepare<kGelu, kRequant, kAct>(d);
   if (rc) return rc;
   const int units = p.total_tiles * p.k_splits;
   // Split-K units write their partials through the pipeline stages' shared
@@ -151,7 +155,7 @@ int gemm_launch(DeviceInfo* d, const CUtensorMap& a, const CUtensorMap& b, const
   if (p.k_splits > 1 && units > d->sms)
     return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "gemm: split-K launch of %d units exceeds the %d SMs", units, d->sms);
   const int grid = units < d->sms ? units : d->sms;
-  fp8_blockwise_gemm_kernel<kGelu, kRequant><<<grid, kGemmThreads, kGemmSmemBytes, stream>>>(a, b, lx, lb, md, mq, p);
+  fp8_blockwise_gemm_kernel<kGelu, kRequant, kAct><<<grid, kGemmThreads, kGemmSmemBytes, stream>>>(a, b, lx, lb, md, mq, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "gemm launch");
   return LTXFP8_OK;
@@ -240,24 +244,24 @@ int gemm_plan_launches(const GemmPlan& g) {
   return (g.split_row0 > 0 ? 1 : 0) + 2;
 }
 
-template <bool kGelu, bool kRequant>
+template <bool kGelu, bool kRequant, int kAct = -1>
 int splitk_reduce_launch(const DeviceInfo* d, const GemmParams& p, cudaStream_t stream) {
   const int64_t groups = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const unsigned blocks = static_cast<unsigned>((groups + 15) / 16);
-  splitk_reduce_kernel<kGelu, kRequant><<<blocks, 256, 0, stream>>>(p);
+  splitk_reduce_kernel<kGelu, kRequant, kAct><<<blocks, 256, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "split-K reduce launch");
   (void)d;
   return LTXFP8_OK;
 }
 
-template <bool kGelu, bool kRequant>
+template <bool kGelu, bool kRequant, int kAct = -1>
 int gemm_launch_full(DeviceInfo* d, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& lx,
                      const CUtensorMap& lb, const CUtensorMap& md, const CUtensorMap& mq, const GemmParams& p,
                      cudaStream_t stream) {
-  int rc = gemm_launch<kGelu, kRequant>(d, a, b, lx, lb, md, mq, p, stream);
+  int rc = gemm_launch<kGelu, kRequant, kAct>(d, a, b, lx, lb, md, mq, p, stream);
   if (rc || p.k_splits == 1) return rc;
-  return splitk_reduce_launch<kGelu, kRequant>(d, p, stream);
+  return splitk_reduce_launch<kGelu, kRequant, kAct>(d, p, stream);
 }
 
 template <bool kGelu, bool kRequant>
@@ -408,18 +412,35 @@ cudaError_t gated_launch(const DeviceInfo* d, cudaStream_t s, const __nv_bfloat1
     }                                                                                              \
   } while (0)
 
+// Warps that share a row: one run of 16 values a thread up to H = 8192, two beyond.
+int norm_warps(int64_t H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
+int norm_block_rows(int64_t H) { return norm_warps(H) > 8 ? 1 : 8 / norm_warps(H); }
+
+template <int kWarps, int kChunks>
+void norm_fwd_launch(const NormFwdParams& p, unsigned grid, cudaStream_t s) {
+  constexpr int kT = norm_threads<kWarps>;
+  if (p.res) {
+    if (p.q) rms_norm_fwd_kernel<kWarps, kChunks, true, true><<<grid, kT, 0, s>>>(p);
+    else rms_norm_fwd_kernel<kWarps, kChunks, true, false><<<grid, kT, 0, s>>>(p);
+  } else {
+    if (p.q) rms_norm_fwd_kernel<kWarps, kChunks, false, true><<<grid, kT, 0, s>>>(p);
+    else rms_norm_fwd_kernel<kWarps, kChunks, false, false><<<grid, kT, 0, s>>>(p);
+  }
+}
+
 }  // namespace
 
 extern "C" {
 
-int ltxfp8_version(void) { return (1 << 16) | 0; }
+int ltxfp8_version(void) { return (1 << 16) | 1; }
 
 const char* ltxfp8_last_error(void) { return t_last_error.c_str(); }
 
 int ltxfp8_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, void* q, int64_t q_ld, float* sfa,
                           int64_t sfa_ld, int flags, void* stream) {
   if (M < 0 || K <= 0 || K % 128 != 0) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize: need K %% 128 == 0, K > 0, M >= 0 (M=%lld K=%lld)", (long long)M, (long long)K);
-  if (flags != LTXFP8_QUANT_TORCH && flags != LTXFP8_QUANT_TRITON) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: unknown mode %d", flags);
+  if (flags != LTXFP8_QUANT_TORCH && flags != LTXFP8_QUANT_TRITON && flags != LTXFP8_QUANT_FINITE)
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: unknown mode %d", flags);
   if (M == 0) return LTXFP8_OK;
   if (!x || !q || !sfa) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: null pointer");
   if (x_ld < K || q_ld < K || sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: leading dimension too small");
@@ -438,6 +459,8 @@ int ltxfp8_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, voi
   auto* qb = static_cast<uint8_t*>(q);
   if (flags == LTXFP8_QUANT_TRITON)
     quant_act_1x128_kernel<kQuantTriton><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
+  else if (flags == LTXFP8_QUANT_FINITE)
+    quant_act_1x128_kernel<kQuantFinite><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
   else
     quant_act_1x128_kernel<kQuantTorch><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
   cudaError_t e = cudaGetLastError();
@@ -826,10 +849,17 @@ int ltxfp8_gelu_tanh_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t
 // offsetting A, sfa, D, the requant outputs and the LoRA rows; N, K, W, sfb and
 // the bias are shared.  split != nullptr: split-K with that plan, partials in
 // the caller's workspace.
+// re != nullptr: the residual epilogue in place of e's GELU and requantisation.
+struct ResidualEpilogue {
+  int act;  // ActKind
+  const __nv_bfloat16* res;
+  int64_t res_ld;
+};
+
 static int gemm_rows(DeviceInfo* d, const void* A, const float* sfa, int64_t sfa_ld, const void* W, const float* sfb,
                      const float* bias, void* D, int64_t M, int64_t N, int64_t K, const ltxfp8_epilogue& e,
                      int64_t row0, int64_t rows, const SplitPlan* split, bool use_pair, cudaStream_t stream,
-                     bool w_fp6 = false) {
+                     bool w_fp6 = false, const ResidualEpilogue* re = nullptr) {
   const bool write_d = !e.skip_d;
   const bool lora = e.lora_ax != nullptr;
   const int tile_m = use_pair ? pair::kTileM : kBM;
@@ -910,6 +940,21 @@ static int gemm_rows(DeviceInfo* d, const void* A, const float* sfa, int64_t sfa
       rc = make_map_2d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.q_out, N, rows, N, 128, 32);
       if (rc) return rc;
     }
+  }
+  if (re) {
+    if (re->res) {
+      p.res = re->res + row0 * re->res_ld;
+      p.res_ld = re->res_ld;
+      p.flags |= kGemmResidual;
+      if (!split) {
+        rc = make_map_2d(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.res, N, rows, re->res_ld * 2, 64, 32);
+        if (rc) return rc;
+      }
+    }
+    if (re->act == kActGeluTanh)
+      return gemm_launch_full<false, false, kActGeluTanh>(d, ma, mb, mlx, mlb, md, mq, p, stream);
+    if (re->act == kActSilu) return gemm_launch_full<false, false, kActSilu>(d, ma, mb, mlx, mlb, md, mq, p, stream);
+    return gemm_launch_full<false, false, kActNone>(d, ma, mb, mlx, mlb, md, mq, p, stream);
   }
   if (use_pair) {
     if (gelu && requant) return gemm_pair_launch<true, true>(d, ma, mb, mlx, mlb, md, mq, p, stream);
@@ -1122,6 +1167,511 @@ int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_
   lora_a_kernel<<<grid, kLoraThreads, smem, static_cast<cudaStream_t>(stream)>>>(mx, ma, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "lora_a launch");
+  return LTXFP8_OK;
+}
+
+// ----------------------------------------------------------------------------- residual epilogue
+int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const void* W, const float* sfb,
+                         const float* bias, const void* residual, int64_t residual_ld, void* D, int64_t M, int64_t N,
+                         int64_t K, int activation, void* workspace, size_t workspace_bytes, void* stream) {
+  if (M < 1 || N < 128 || K < 128 || N % 128 != 0 || K % 128 != 0)
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE,
+                "gemm_residual: need M >= 1 and N, K positive multiples of 128 (M=%lld N=%lld K=%lld)", (long long)M,
+                (long long)N, (long long)K);
+  if (M > 0x7FFFFFFF || N > 0x7FFFFFFF || K > 0x7FFFFFFF)
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "gemm_residual: dimension exceeds int32");
+  if (activation < LTXFP8_ACT_NONE || activation > LTXFP8_ACT_SILU)
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: unknown activation %d", activation);
+  if (!A || !sfa || !W || !sfb || !D) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: null operand");
+  if (sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: sfa_ld < M");
+  if (residual && residual_ld < N) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: residual_ld < N");
+  if (!aligned(A, 16) || !aligned(W, 16) || !aligned(D, 16) || (bias && !aligned(bias, 16)))
+    return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: A, W, D and bias must be 16-byte aligned");
+  if (!aligned(sfa, 4) || !aligned(sfb, 4)) return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: scales must be 4-byte aligned");
+  if (residual && (!aligned(residual, 16) || residual_ld % 8 != 0))
+    return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: residual must be 16-byte aligned with residual_ld %% 8 == 0");
+  DeviceInfo* d;
+  int rc = device_info(&d);
+  if (rc) return rc;
+  ltxfp8_epilogue e;
+  memset(&e, 0, sizeof(e));
+  e.workspace = workspace;
+  e.workspace_bytes = workspace_bytes;
+  const ResidualEpilogue re{activation, static_cast<const __nv_bfloat16*>(residual), residual_ld};
+  auto s = static_cast<cudaStream_t>(stream);
+  const GemmPlan g = gemm_plan(d->sms, M, N, K);
+  const size_t need = splitk_bytes(g);
+  if (need == 0 || !workspace || need > workspace_bytes)
+    return gemm_rows(d, A, sfa, sfa_ld, W, sfb, bias, D, M, N, K, e, 0, M, nullptr, false, s, false, &re);
+  if (!aligned(workspace, 16)) return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: workspace must be 16-byte aligned");
+  if (g.split_row0 > 0) {
+    rc = gemm_rows(d, A, sfa, sfa_ld, W, sfb, bias, D, M, N, K, e, 0, g.split_row0, nullptr, false, s, false, &re);
+    if (rc) return rc;
+  }
+  return gemm_rows(d, A, sfa, sfa_ld, W, sfb, bias, D, M, N, K, e, g.split_row0, M - g.split_row0, &g.split, false, s,
+                   false, &re);
+}
+
+// ----------------------------------------------------------------------------- residual RMS norm
+constexpr int64_t kNormMaxH = 16384;
+
+static int norm_check(const char* name, int64_t M, int64_t H, const void* weight, int weight_dtype) {
+  if (M < 0 || H <= 0 || H % 128 != 0 || H > kNormMaxH)
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: need H %% 128 == 0, 0 < H <= %lld, M >= 0 (M=%lld H=%lld)", name,
+                (long long)kNormMaxH, (long long)M, (long long)H);
+  if (M > 0x7FFFFFFF) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: too many rows", name);
+  if (weight && weight_dtype != LTXFP8_DTYPE_F32 && weight_dtype != LTXFP8_DTYPE_BF16)
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: weight must be fp32 or bf16", name);
+  if (weight && !aligned(weight, 16)) return fail(LTXFP8_ERR_MISALIGNED, "%s: weight must be 16-byte aligned", name);
+  return LTXFP8_OK;
+}
+
+// A row operand: 16-byte aligned rows of at least H values.
+static int norm_rows(const char* name, const char* what, const void* p, int64_t ld, int64_t H) {
+  if (!p) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: %s is null", name, what);
+  if (ld < H) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the row stride of %s is below %lld", name, what, (long long)H);
+  if (!aligned(p, 16) || ld % 8 != 0)
+    return fail(LTXFP8_ERR_MISALIGNED, "%s: %s must be 16-byte aligned with a row stride %% 8 == 0", name, what);
+  return LTXFP8_OK;
+}
+
+int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t M,
+                             int64_t H, const void* weight, int weight_dtype, float eps, void* h, void* q, float* sfa,
+                             int64_t sfa_ld, void* out, float* rstd, void* stream) {
+  const char* name = "rms_norm_quantize";
+  int rc = norm_check(name, M, H, weight, weight_dtype);
+  if (rc) return rc;
+  if (!(eps >= 0.0f)) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", name);
+  if (M == 0) return LTXFP8_OK;
+  if ((rc = norm_rows(name, "x", x, x_ld, H)) != 0) return rc;
+  if (residual) {
+    if ((rc = norm_rows(name, "residual", residual, residual_ld, H)) != 0) return rc;
+    if ((rc = norm_rows(name, "h", h, H, H)) != 0) return rc;
+  } else if (h) {
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: h is only written with a residual", name);
+  }
+  if (q) {
+    if (out) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: q and out exclude each other", name);
+    if (!sfa || sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: sfa is null or sfa_ld < M", name);
+    if (!aligned(q, 16) || !aligned(sfa, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: q must be 16-byte aligned", name);
+  } else {
+    if ((rc = norm_rows(name, "out", out, H, H)) != 0) return rc;
+  }
+  if (rstd && !aligned(rstd, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: rstd must be 4-byte aligned", name);
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  NormFwdParams p;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.res = static_cast<const __nv_bfloat16*>(residual);
+  p.x_ld = x_ld;
+  p.res_ld = residual_ld;
+  p.M = M;
+  p.H = static_cast<int>(H);
+  p.w = weight;
+  p.w_f32 = weight_dtype == LTXFP8_DTYPE_F32;
+  p.eps = eps;
+  p.h = static_cast<__nv_bfloat16*>(h);
+  p.q = static_cast<uint8_t*>(q);
+  p.sfa = sfa;
+  p.sfa_ld = sfa_ld;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.rstd = rstd;
+  const int rows = norm_block_rows(H);
+  const unsigned grid = static_cast<unsigned>((M + rows - 1) / rows);
+  auto s = static_cast<cudaStream_t>(stream);
+  switch (norm_warps(H)) {
+    case 1: norm_fwd_launch<1, 1>(p, grid, s); break;
+    case 2: norm_fwd_launch<2, 1>(p, grid, s); break;
+    case 4: norm_fwd_launch<4, 1>(p, grid, s); break;
+    case 8: norm_fwd_launch<8, 1>(p, grid, s); break;
+    default:
+      if (H <= 8192) norm_fwd_launch<16, 1>(p, grid, s);
+      else norm_fwd_launch<16, 2>(p, grid, s);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "rms_norm_quantize launch");
+  return LTXFP8_OK;
+}
+
+// Blocks of the norm's backward: each SM's share of resident blocks, at most one per row group.
+static int64_t norm_bwd_blocks(int sms, int64_t M, int64_t H) {
+  const int rows = norm_block_rows(H);
+  const int64_t groups = (M + rows - 1) / rows;
+  const int64_t cap = static_cast<int64_t>(sms) * (norm_warps(H) > 8 ? 2 : 4);
+  return groups < cap ? groups : cap;
+}
+
+int ltxfp8_rms_norm_backward_workspace_bytes(int64_t M, int64_t H, size_t* bytes) {
+  if (!bytes) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "rms_norm_backward: null pointer");
+  *bytes = 0;
+  int rc = norm_check("rms_norm_backward", M, H, nullptr, 0);
+  if (rc) return rc;
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  *bytes = static_cast<size_t>(norm_bwd_blocks(d->sms, M, H)) * static_cast<size_t>(H) * 4u;
+  return LTXFP8_OK;
+}
+
+int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64_t h_ld, const float* rstd,
+                             const void* weight, int weight_dtype, const void* dh, int64_t dh_ld, int64_t M, int64_t H,
+                             void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "rms_norm_backward";
+  int rc = norm_check(name, M, H, weight, weight_dtype);
+  if (rc) return rc;
+  if (dweight && !weight) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: dweight without a weight", name);
+  auto s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (dweight) {
+      cudaError_t e = cudaMemsetAsync(dweight, 0, static_cast<size_t>(H) * (weight_dtype == LTXFP8_DTYPE_F32 ? 4 : 2), s);
+      if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward clear");
+    }
+    return LTXFP8_OK;
+  }
+  if ((rc = norm_rows(name, "dy", dy, dy_ld, H)) != 0) return rc;
+  if ((rc = norm_rows(name, "h", h, h_ld, H)) != 0) return rc;
+  if (dh && (rc = norm_rows(name, "dh", dh, dh_ld, H)) != 0) return rc;
+  if ((rc = norm_rows(name, "dx", dx, H, H)) != 0) return rc;
+  if (!rstd) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: rstd is null", name);
+  if (!aligned(rstd, 4) || (dweight && !aligned(dweight, 4)))
+    return fail(LTXFP8_ERR_MISALIGNED, "%s: rstd and dweight must be 4-byte aligned", name);
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  const int64_t blocks = norm_bwd_blocks(d->sms, M, H);
+  if (dweight) {
+    if (!workspace || workspace_bytes < static_cast<size_t>(blocks) * static_cast<size_t>(H) * 4u)
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the workspace is missing or too small", name);
+    if (!aligned(workspace, 16)) return fail(LTXFP8_ERR_MISALIGNED, "%s: workspace must be 16-byte aligned", name);
+  }
+  NormBwdParams p;
+  p.dy = static_cast<const __nv_bfloat16*>(dy);
+  p.h = static_cast<const __nv_bfloat16*>(h);
+  p.dh = static_cast<const __nv_bfloat16*>(dh);
+  p.dy_ld = dy_ld;
+  p.h_ld = h_ld;
+  p.dh_ld = dh_ld;
+  p.M = M;
+  p.H = static_cast<int>(H);
+  p.rstd = rstd;
+  p.w = weight;
+  p.w_f32 = weight_dtype == LTXFP8_DTYPE_F32;
+  p.dx = static_cast<__nv_bfloat16*>(dx);
+  p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  switch (norm_warps(H)) {
+    case 1: rms_norm_bwd_kernel<1, 1><<<grid, 256, 0, s>>>(p); break;
+    case 2: rms_norm_bwd_kernel<2, 1><<<grid, 256, 0, s>>>(p); break;
+    case 4: rms_norm_bwd_kernel<4, 1><<<grid, 256, 0, s>>>(p); break;
+    case 8: rms_norm_bwd_kernel<8, 1><<<grid, 256, 0, s>>>(p); break;
+    default:
+      if (H <= 8192) rms_norm_bwd_kernel<16, 1><<<grid, 512, 0, s>>>(p);
+      else rms_norm_bwd_kernel<16, 2><<<grid, 512, 0, s>>>(p);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward launch");
+  if (dweight) {
+    col_sum_kernel<<<static_cast<unsigned>((H + 31) / 32), 256, 0, s>>>(p.dw_part, static_cast<int>(blocks),
+                                                                        static_cast<int>(H), dweight,
+                                                                        weight_dtype == LTXFP8_DTYPE_F32);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward sum launch");
+  }
+  return LTXFP8_OK;
+}
+
+// ----------------------------------------------------------------------------- activation checkpoints
+static int act_check(const char* name, int64_t M, int64_t N, int activation) {
+  if (M < 0 || N <= 0 || N % 128 != 0 || M > 0x7FFFFFFF || N > (static_cast<int64_t>(1) << 22))
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: need N %% 128 == 0, 0 < N <= 2^22, 0 <= M < 2^31 (M=%lld N=%lld)", name,
+                (long long)M, (long long)N);
+  if (activation != LTXFP8_ACT_GELU_TANH && activation != LTXFP8_ACT_SILU)
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", name, activation);
+  return LTXFP8_OK;
+}
+
+static int act_codes(const char* name, const char* what, const void* q, const float* s, int64_t ld, int64_t M) {
+  if (!q || !s) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the codes or scales of %s are null", name, what);
+  if (ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the scale stride of %s is below M", name, what);
+  if (!aligned(q, 16) || !aligned(s, 4))
+    return fail(LTXFP8_ERR_MISALIGNED, "%s: the codes of %s must be 16-byte aligned", name, what);
+  return LTXFP8_OK;
+}
+
+int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, int activation, void* yq, float* ys,
+                             int64_t ys_ld, void* zq, float* zs, int64_t zs_ld, void* stream) {
+  const char* name = "act_quantize_save";
+  int rc = act_check(name, M, N, activation);
+  if (rc) return rc;
+  if (M == 0) return LTXFP8_OK;
+  if ((rc = norm_rows(name, "z", z, z_ld, N)) != 0) return rc;
+  if ((rc = act_codes(name, "y", yq, ys, ys_ld, M)) != 0) return rc;
+  if ((rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
+  const int64_t groups = N / 128;
+  const int64_t blocks = (M * groups + kActSaveGroups - 1) / kActSaveGroups;
+  if (blocks > 0x7FFFFFFF) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: M * N is too large", name);
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  ActSaveParams p;
+  p.z = static_cast<const __nv_bfloat16*>(z);
+  p.z_ld = z_ld;
+  p.M = M;
+  p.N = N;
+  p.groups = static_cast<uint32_t>(groups);
+  p.magic = static_cast<uint32_t>(((1ull << 32) + groups - 1) / static_cast<uint64_t>(groups));
+  p.yq = static_cast<uint8_t*>(yq);
+  p.ys = ys;
+  p.ys_ld = ys_ld;
+  p.zq = static_cast<uint8_t*>(zq);
+  p.zs = zs;
+  p.zs_ld = zs_ld;
+  auto s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (activation == LTXFP8_ACT_GELU_TANH) act_quantize_save_kernel<kActGeluTanh><<<grid, 256, 0, s>>>(p);
+  else act_quantize_save_kernel<kActSilu><<<grid, 256, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "act_quantize_save launch");
+  return LTXFP8_OK;
+}
+
+// Row shares of the activation's backward: enough blocks for several per SM.
+static dim3 act_bwd_grid(int sms, int64_t M, int64_t N) {
+  const int64_t groups = N / 128;
+  const int kg = groups >= 4 ? 4 : 1;
+  const int64_t gx = (groups + kg - 1) / kg;
+  const int64_t passes = (M + 32 / kg * kActBwdUnroll - 1) / (32 / kg * kActBwdUnroll);
+  int64_t gy = (static_cast<int64_t>(sms) * 8 + gx - 1) / gx;
+  if (gy > passes) gy = passes;
+  if (gy > 65535) gy = 65535;
+  if (gy < 1) gy = 1;
+  return dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+}
+
+int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
+  if (!bytes) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "act_backward: null pointer");
+  *bytes = 0;
+  int rc = act_check("act_backward", M, N, LTXFP8_ACT_SILU);
+  if (rc) return rc;
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  *bytes = static_cast<size_t>(act_bwd_grid(d->sms, M, N).y) * static_cast<size_t>(N) * 4u;
+  return LTXFP8_OK;
+}
+
+int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const float* zs, int64_t zs_ld, int64_t M,
+                        int64_t N, int activation, void* dz, void* dzq, float* dzs, int64_t dzs_ld, float* dbias,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "act_backward";
+  int rc = act_check(name, M, N, activation);
+  if (rc) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (dbias) {
+      cudaError_t e = cudaMemsetAsync(dbias, 0, static_cast<size_t>(N) * 4u, s);
+      if (e != cudaSuccess) return cuda_fail(e, "act_backward clear");
+    }
+    return LTXFP8_OK;
+  }
+  if ((rc = norm_rows(name, "dy", dy, dy_ld, N)) != 0) return rc;
+  if ((rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
+  if (!dz && !dzq) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: need dz or dzq", name);
+  if (dz && (rc = norm_rows(name, "dz", dz, N, N)) != 0) return rc;
+  if (dzq && (rc = act_codes(name, "dz", dzq, dzs, dzs_ld, M)) != 0) return rc;
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  const dim3 grid = act_bwd_grid(d->sms, M, N);
+  if (dbias) {
+    if (!workspace || workspace_bytes < static_cast<size_t>(grid.y) * static_cast<size_t>(N) * 4u)
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the workspace is missing or too small", name);
+    if (!aligned(workspace, 16) || !aligned(dbias, 4))
+      return fail(LTXFP8_ERR_MISALIGNED, "%s: workspace must be 16-byte, dbias 4-byte aligned", name);
+  }
+  ActBwdParams p;
+  p.dy = static_cast<const __nv_bfloat16*>(dy);
+  p.dy_ld = dy_ld;
+  p.M = M;
+  p.N = N;
+  p.zq = static_cast<const uint8_t*>(zq);
+  p.zs = zs;
+  p.zs_ld = zs_ld;
+  p.groups = static_cast<int>(N / 128);
+  p.dz = static_cast<__nv_bfloat16*>(dz);
+  p.dzq = static_cast<uint8_t*>(dzq);
+  p.dzs = dzs;
+  p.dzs_ld = dzs_ld;
+  p.db_part = dbias ? static_cast<float*>(workspace) : nullptr;
+  const bool gelu = activation == LTXFP8_ACT_GELU_TANH;
+  if (N >= 512) {
+    if (gelu) act_backward_kernel<kActGeluTanh, 4><<<grid, 256, 0, s>>>(p);
+    else act_backward_kernel<kActSilu, 4><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (gelu) act_backward_kernel<kActGeluTanh, 1><<<grid, 256, 0, s>>>(p);
+    else act_backward_kernel<kActSilu, 1><<<grid, 256, 0, s>>>(p);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "act_backward launch");
+  if (dbias) {
+    col_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), 256, 0, s>>>(p.db_part, static_cast<int>(grid.y),
+                                                                        static_cast<int>(N), dbias, true);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "act_backward sum launch");
+  }
+  return LTXFP8_OK;
+}
+
+int ltxfp8_transpose_weight_128x128(const void* q, const float* sfb, int64_t N, int64_t K, void* qt, float* sfbt,
+                                    void* stream) {
+  if (N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0 || N / 128 > 65535)
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "transpose_weight: N and K must be positive multiples of 128 (N=%lld K=%lld)",
+                (long long)N, (long long)K);
+  if (!q || !sfb || !qt || !sfbt) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "transpose_weight: null pointer");
+  if (q == qt) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "transpose_weight: not in place");
+  if (!aligned(q, 16) || !aligned(qt, 16) || !aligned(sfb, 4) || !aligned(sfbt, 4))
+    return fail(LTXFP8_ERR_MISALIGNED, "transpose_weight: q and qt must be 16-byte aligned");
+  DeviceInfo* d;
+  int rc = device_info(&d);
+  if (rc) return rc;
+  transpose_weight_kernel<<<dim3(static_cast<unsigned>(K / 128), static_cast<unsigned>(N / 128)), 256, 0,
+                            static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(q), sfb, N, K,
+                                                                 static_cast<uint8_t*>(qt), sfbt);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "transpose_weight launch");
+  return LTXFP8_OK;
+}
+
+// ----------------------------------------------------------------------------- weight gradient
+// Tile width and splits of the summed axis.  A cost model in clock cycles picks among tile
+// widths (multiples of 16, at most 256; a single tile when N fits one) and splits: a stage
+// of 64 tokens costs the larger of its MMAs (4 cycles a column) and the expansion of its
+// codes, a unit has a fixed start and drain, and the units run in waves over the SMs; split
+// partials are written and read back at L2 rates and cost one more launch.
+struct WgradPlan {
+  int nt, n_tiles, k_tiles, stages, splits, per_split;
+  size_t ws_bytes;
+};
+
+static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
+  WgradPlan best{};
+  double best_cost = 0.0;
+  const int64_t stages = (M + kWgStageM - 1) / kWgStageM, k_tiles = (K + kWgTileK - 1) / kWgTileK;
+  const int nt_hi = static_cast<int>(N < 256 ? N : 256), nt_lo = N <= 256 ? nt_hi : 128;
+  for (int nt = nt_hi; nt >= nt_lo; nt -= 16) {
+    const int64_t n_tiles = (N + nt - 1) / nt, tiles = n_tiles * k_tiles;
+    const int64_t max_s = stages < 64 ? stages : 64;
+    for (int64_t s = 1; s <= max_s; ++s) {
+      const int64_t per = (stages + s - 1) / s, used = (stages + per - 1) / per;
+      if (used != s) continue;
+      const double stage = 4.0 * nt > 700.0 ? 4.0 * nt : 700.0;
+      const double unit = static_cast<double>(per) * stage + 3000.0 + 16.0 * nt;
+      const int64_t waves = (tiles * s + sms - 1) / sms;
+      const double ws = s > 1 ? static_cast<double>(tiles * s) * nt * kWgTileK * 4.0 : 0.0;
+      const double cost = static_cast<double>(waves) * unit + (s > 1 ? 5000.0 + ws / 1500.0 : 0.0);
+      if (ws <= 512.0 * 1048576.0 && tiles * s <= 0x7FFFFFFF && (best.nt == 0 || cost < best_cost)) {
+        best_cost = cost;
+        best = WgradPlan{nt, static_cast<int>(n_tiles), static_cast<int>(k_tiles), static_cast<int>(stages),
+                         static_cast<int>(s), static_cast<int>(per), static_cast<size_t>(ws)};
+      }
+    }
+  }
+  return best;
+}
+
+static int wgrad_check(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N <= 0 || K <= 0 || N % 16 != 0 || K % 128 != 0 || M > 0x7FFFFF00 || N > (1 << 20) || K > (1 << 20))
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE,
+                "wgrad: need M >= 0, N a multiple of 16 and K of 128, both in (0, 2^20] (M=%lld N=%lld K=%lld)",
+                (long long)M, (long long)N, (long long)K);
+  return LTXFP8_OK;
+}
+
+int ltxfp8_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes) {
+  if (!bytes) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad: null pointer");
+  *bytes = 0;
+  int rc = wgrad_check(M, N, K);
+  if (rc || M == 0) return rc;
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  *bytes = wgrad_plan(d->sms, M, N, K).ws_bytes;
+  return LTXFP8_OK;
+}
+
+int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const float* xs, int64_t xs_ld, float alpha,
+                 void* out, int transposed, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  int rc = wgrad_check(M, N, K);
+  if (rc) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (!out) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad: out is null");
+  if (!aligned(out, 16)) return fail(LTXFP8_ERR_MISALIGNED, "wgrad: out must be 16-byte aligned");
+  if (M == 0) {
+    cudaError_t e = cudaMemsetAsync(out, 0, static_cast<size_t>(N) * static_cast<size_t>(K) * 2u, s);
+    if (e != cudaSuccess) return cuda_fail(e, "wgrad clear");
+    return LTXFP8_OK;
+  }
+  if (!g || !x) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad: null operand");
+  if (g_ld < N || x_ld < K || (xs && xs_ld < M)) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad: leading dimension too small");
+  if (!aligned(g, 16) || !aligned(x, 16) || g_ld % 8 != 0 || x_ld % (xs ? 16 : 8) != 0 || (xs && !aligned(xs, 4)))
+    return fail(LTXFP8_ERR_MISALIGNED, "wgrad: g and x must be 16-byte aligned with 16-byte row strides");
+  DeviceInfo* d;
+  rc = device_info(&d);
+  if (rc) return rc;
+  const WgradPlan pl = wgrad_plan(d->sms, M, N, K);
+  if (pl.ws_bytes) {
+    if (!workspace || workspace_bytes < pl.ws_bytes)
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad: the workspace is missing or too small");
+    if (!aligned(workspace, 16)) return fail(LTXFP8_ERR_MISALIGNED, "wgrad: workspace must be 16-byte aligned");
+  }
+  const bool fp8 = xs != nullptr;
+  CUtensorMap mx, mg;
+  if (fp8) rc = make_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, K, M, x_ld, 128, kWgStageM);
+  else rc = make_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, M, x_ld * 2, 64, kWgStageM);
+  if (rc) return rc;
+  rc = make_map_2d(&mg, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g, N, M, g_ld * 2, 64, kWgStageM);
+  if (rc) return rc;
+  WgradParams p;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.stages = pl.stages;
+  p.stages_per_split = pl.per_split;
+  p.splits = pl.splits;
+  p.k_tiles = pl.k_tiles;
+  p.n_tiles = pl.n_tiles;
+  p.nt = pl.nt;
+  p.groups = static_cast<int>(K / 128);
+  p.xs = xs;
+  p.xs_ld = xs_ld;
+  p.alpha = alpha;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ld_n = transposed ? 1 : K;
+  p.ld_k = transposed ? N : 1;
+  p.ws = static_cast<float*>(workspace);
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!d->wgrad_ready[fp8]) {
+      cudaError_t e = fp8 ? cudaFuncSetAttribute(wgrad_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmemBytes)
+                          : cudaFuncSetAttribute(wgrad_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmemBytes);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(wgrad smem)");
+      d->wgrad_ready[fp8] = true;
+    }
+  }
+  const int units = pl.k_tiles * pl.n_tiles * pl.splits;
+  const int grid = units < d->sms ? units : d->sms;
+  if (fp8) wgrad_kernel<true><<<grid, kWgThreads, kWgSmemBytes, s>>>(mx, mg, p);
+  else wgrad_kernel<false><<<grid, kWgThreads, kWgSmemBytes, s>>>(mx, mg, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "wgrad launch");
+  if (pl.splits > 1) {
+    const int64_t threads = static_cast<int64_t>(pl.k_tiles) * pl.n_tiles * pl.nt * (kWgTileK / 4);
+    wgrad_reduce_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "wgrad reduce launch");
+  }
   return LTXFP8_OK;
 }
 

@@ -164,7 +164,7 @@ __device__ __forceinline__ void quant_group8(const float (&f)[8], bool valid, ui
   }
   float s, inv;
   group_scale<kMode>(amax, s, inv);
-  const bool in_range = (kMode == kQuantTriton) || isfinite(s);
+  const bool in_range = (kMode != kQuantTorch) || isfinite(s);
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {

@@ -199,6 +199,20 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_addr) {
   return d;
 }
 
+// Descriptor of an MN-major 16-bit operand (rows of 64 M/N values = 128 bytes, one row per
+// K index, 128 B swizzle): an atom is 64 MN x 8 K values (1024 B), the next 8 K values
+// 1024 B further (stride byte offset), the next 64 M/N values `mn_stride` bytes further
+// (leading byte offset).  A TMA box of 64 values x R rows lands as R / 8 such atoms.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint32_t mn_stride) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(mn_stride >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
 // Instruction descriptor: dense, f32 accumulator, K-major A and B, M x N.
 // a/b format: kind::f8f6f4 E4M3 = 0; kind::f16 BF16 = 1.
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t ab_format, uint32_t m, uint32_t n) {
@@ -208,6 +222,10 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t ab_format, uint32_t m
          | ((n >> 3) << 17)             // N >> 3
          | ((m >> 4) << 24);            // M >> 4
 }
+
+// Instruction descriptor bits: A / B are MN-major ("transposed") instead of K-major.
+constexpr uint32_t kIdescAMnMajor = 1u << 15;
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
 
 // kind::f8f6f4 operand formats (instruction descriptor bits 7-9 for A, 10-12 for B).
 constexpr uint32_t kFmtE4M3 = 0u;

@@ -11,7 +11,14 @@ namespace ltxfp8 {
 enum QuantMode : int {
   kQuantTorch = 0,   // s = (1/amax)*448 with IEEE roundings, NaN-propagating amax (functional.py:138-144)
   kQuantTriton = 1,  // s = 448/amax and 1/s via div.full.f32, NaN-ignoring amax (triton_ops.py:13-22)
+  // scale = amax * (1/448) and s = 1/scale (approximate reciprocal, within 1 ulp),
+  // NaN-propagating amax, amax floored at 448 * 2^-126: an all-zero group (a padded
+  // token) gets zero codes and a normal scale where the two reference arithmetics
+  // give NaN codes.
+  kQuantFinite = 2,
 };
+
+constexpr float kFiniteAmaxMin = 448.0f * 1.1754945e-38f;  // a little above 448 * 2^-126
 
 constexpr int kQuantRowsPerBlock = 16;   // 16 lanes per 128-group, 16 groups per 256-thread block
 constexpr int kQuantGroupsPerThread = 4; // groups in flight per thread (4 x 16 B loads)
@@ -23,6 +30,9 @@ __device__ __forceinline__ void group_scale(float amax, float& s, float& inv) {
   if constexpr (kMode == kQuantTriton) {
     s = div_full(448.0f, amax);
     inv = div_full(1.0f, s);
+  } else if constexpr (kMode == kQuantFinite) {
+    inv = __fmul_rn(fmax_nan(amax, kFiniteAmaxMin), 1.0f / 448.0f);
+    s = rcp_approx(inv);  // inv is in [2^-126, 2^128 / 448]: neither it nor 1/inv is subnormal
   } else {
     s = __fmul_rn(__frcp_rn(amax), 448.0f);
     inv = __frcp_rn(s);
@@ -73,7 +83,7 @@ __global__ void __launch_bounds__(256) quant_act_1x128_kernel(const __nv_bfloat1
     // A finite scale keeps every |x * s| <= 448, where the saturating hardware
     // conversion equals torch's; only non-finite scales need torch's overflow-to-NaN
     // patch.  The Triton kernel converts with the saturating instruction throughout.
-    const bool in_range = (kMode == kQuantTriton) || isfinite(s);
+    const bool in_range = (kMode != kQuantTorch) || isfinite(s);
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

@@ -23,6 +23,7 @@ ERR_DEVICE_STATUS = -6
 
 QUANT_TORCH = 0
 QUANT_TRITON = 1
+QUANT_FINITE = 2  # scale = amax / 448, all-zero groups quantise to zeros
 
 GELU_NONE = 0
 GELU_TANH = 1       # torch's CUDA GELU-tanh formula (bit-identical bf16 results)
@@ -31,6 +32,10 @@ GELU_TANH_FAST = 2  # x / (1 + 2^a) with approximate instructions (within one bf
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+
+ACT_NONE = 0
+ACT_GELU_TANH = 1
+ACT_SILU = 2
 
 _lock = threading.Lock()
 _lib = None
@@ -72,6 +77,7 @@ class GemmPlanInfo(ctypes.Structure):
 
 # name -> (restype, argtypes); the exported symbols of include/ltxfp8.h
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_sz = ctypes.c_size_t
 SIGNATURES = {
     "ltxfp8_version": (_i32, []),
     "ltxfp8_last_error": (ctypes.c_char_p, []),
@@ -101,6 +107,20 @@ SIGNATURES = {
     "ltxfp8_fp6_to_tc": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     "ltxfp8_gemm_static_scratch": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                            ctypes.POINTER(Epilogue), _vp]),
+    "ltxfp8_rms_norm_quantize": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp,
+                                        _vp, _vp]),
+    "ltxfp8_rms_norm_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp,
+                                        _sz, _vp]),
+    "ltxfp8_rms_norm_backward_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_sz)]),
+    "ltxfp8_gemm_residual": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _sz,
+                                    _vp]),
+    "ltxfp8_act_quantize_save": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "ltxfp8_act_backward": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _sz,
+                                   _vp]),
+    "ltxfp8_act_backward_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_sz)]),
+    "ltxfp8_wgrad": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _f32, _vp, _i32, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "ltxfp8_wgrad_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "ltxfp8_transpose_weight_128x128": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     "ltxfp8_device_status": (_i32, [ctypes.POINTER(ctypes.c_uint), _i32, _vp]),
     "ltxfp8_selftest_wait_timeout": (_i32, [ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_uint), _vp]),
 }
