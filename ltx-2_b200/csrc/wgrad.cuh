@@ -15,8 +15,8 @@
 //   warp 0      TMA producer: codes [64, 256] (16 KB) into the raw ring, g [64, nt] into its
 //               own ring (bf16 x: straight into the operand ring)
 //   warp 1      MMA issuer: 2 x 4 MMAs (M128 N=nt K16) a stage
-//   warps 4-11  expand the raw codes into the swizzled MN-major operand tile; after the
-//               unit's last stage, drain the accumulators
+//   warps 4-19  two groups of 8 that expand alternate stages of raw codes into the swizzled
+//               MN-major operand tile; after the unit's last stage, all drain the accumulators
 // The summed axis is divided among `splits` units where the tiles alone would not fill the
 // GPU; those write fp32 partials that wgrad_reduce_kernel adds in split order.
 #pragma once
@@ -27,7 +27,8 @@ namespace ltxfp8 {
 
 constexpr int kWgTileK = 256;
 constexpr int kWgStageM = 64;
-constexpr int kWgThreads = 384;
+constexpr int kWgGroups = 2;        // expanding warp groups; stage i belongs to group i % 2
+constexpr int kWgThreads = 128 + kWgGroups * 256;
 constexpr int kWgRawStages = 4;   // 16 KB each
 constexpr int kWgGStages = 3;     // 32 KB each
 constexpr int kWgOpStages = 2;    // 32 KB each (3 when x is bf16: no raw ring)
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
       mbar_init(&op_empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
+    mbar_init(acc_empty, kWgGroups * 8);
     mbar_init(drain, 1);
     fence_mbarrier_init();
   }
@@ -232,9 +233,9 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     mbar_wait(drain, 0u, kStWgDrain);
   } else if (warp >= 4) {
     // -------------------------------------------------------------- expansion, epilogue
-    const int t = static_cast<int>(threadIdx.x) - 128;
+    const int t = (static_cast<int>(threadIdx.x) - 128) & 255, grp = (warp - 4) >> 3;
     const int c = t & 7, rsub = t >> 3;  // 16-code chunk of a 128-code row, row modulo 32
-    const int sp = warp & 3, half = (warp - 4) >> 2;
+    const int sp = warp & 3, half = ((warp - 4) >> 2) & 1;
     uint32_t it = 0, tcount = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++tcount) {
@@ -250,9 +251,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           }
         };
         float sc[4], nx[4];
-        load_scales(0, sc);
-        for (int i = 0; i < w.count; ++i, ++it) {
-          load_scales(i + 1, nx);
+        int i = static_cast<int>(it + grp) & (kWgGroups - 1);  // this group's first stage of the unit
+        load_scales(i, sc);
+        const uint32_t it0 = it;
+        for (; i < w.count; i += kWgGroups) {
+          it = it0 + i;
+          load_scales(i + kWgGroups, nx);
           const uint32_t sr = it % kWgRawStages, pr = (it / kWgRawStages) & 1u;
           const uint32_t so = it % kOpStages, po = (it / kOpStages) & 1u;
           if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[sr], pr, kStWgConvert)) ||
@@ -287,6 +291,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           for (int j = 0; j < 4; ++j) sc[j] = nx[j];
         }
         if (!ok) break;
+        it = it0 + w.count;
       }
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full, tcount & 1u, kStWgAccFull))) {
         ok = false;
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
       const bool k_ok = w.k0 + half * 128 < p.K;  // warp-uniform: K % 128 == 0
       if (k_ok) {
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sp * 32) << 16) + half * 256;
-        for (int c0 = 0; c0 < p.nt; c0 += 32) {  // columns past nt are stale and not stored
+        for (int c0 = grp * 32; c0 < p.nt; c0 += 32 * kWgGroups) {  // columns past nt are stale and not stored
           uint32_t r[32];
           tmem_ld_32x32b_x32(taddr + c0, r);
           tmem_wait_ld();

@@ -129,6 +129,8 @@ SIGNATURES = {
 def load(path: str | None = None):
     """Load (once) and return the ctypes handle of libltxfp8.so."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             p = path or LIB_PATH

@@ -25,7 +25,9 @@ def align4(n: int) -> int:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # The raw handle of torch.cuda.current_stream(t.device), without building a Stream object
+    # (2.2 us a call).
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _require_cuda(name: str, *ts: Optional[torch.Tensor]) -> None:
@@ -46,13 +48,15 @@ def _require_cuda(name: str, *ts: Optional[torch.Tensor]) -> None:
 class _DeviceGuard:
     """Switch to the tensor's device only when it differs from the current one."""
 
+    __slots__ = ("idx", "prev")
+
     def __init__(self, t: torch.Tensor):
-        self.idx = t.device.index
+        self.idx = t.get_device()
         self.prev = None
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
-        if self.idx is not None and self.idx != cur:
+        cur = torch._C._cuda_getDevice()  # a CUDA tensor exists: CUDA is initialised
+        if self.idx != cur:
             self.prev = cur
             torch.cuda.set_device(self.idx)
 
@@ -551,6 +555,8 @@ def _bf16_rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """bf16 [..., K] as an [M, K] matrix with 16-byte aligned rows (a copy only where it has none)."""
     if x.dtype != torch.bfloat16:
         raise RuntimeError(f"{name}: expected bf16, got {x.dtype}")
+    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0 and x.shape[1] % 8 == 0 and x.shape[1]:
+        return x
     if x.dim() < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"{name}: expected a [..., K] tensor, got shape {tuple(x.shape)}")
     x2 = x.reshape(-1, x.shape[-1])
@@ -558,6 +564,11 @@ def _bf16_rows(x: torch.Tensor, name: str) -> torch.Tensor:
     if M > 0 and (x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (x2.stride(0) % 8 or x2.stride(0) < K))):
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
+
+
+def _new(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """torch.empty((M, N)): the strided form parses its arguments faster (1.5 against 2.3 us)."""
+    return torch.empty_strided((M, N), (N, 1), dtype=dtype, device=device)
 
 
 def _ld(x2: torch.Tensor) -> int:
@@ -570,7 +581,7 @@ def _code_rows(q: torch.Tensor, scales: torch.Tensor, name: str) -> Tuple[torch.
         raise RuntimeError(f"{name}: codes must be float8_e4m3fn, got {q.dtype}")
     if q.dim() < 1 or q.shape[-1] == 0 or q.shape[-1] % 128:
         raise RuntimeError(f"{name}: expected [..., K] codes with K a positive multiple of 128, got {tuple(q.shape)}")
-    q2 = q.reshape(-1, q.shape[-1]).contiguous()
+    q2 = q if q.dim() == 2 and q.is_contiguous() else q.reshape(-1, q.shape[-1]).contiguous()
     if q2.data_ptr() % 16:
         q2 = q2.clone()
     M, K = q2.shape
@@ -604,7 +615,7 @@ def _workspace(fn: str, dims: Tuple[int, ...], device) -> Tuple[Optional[torch.T
         b = ctypes.c_size_t(0)
         L.check(getattr(L.load(), fn)(*dims, ctypes.byref(b)))
         n = _TRAIN_WS_CACHE[key] = b.value
-    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+    return (torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device) if n else None), n
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -626,15 +637,15 @@ def rms_norm_quantize(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
             raise RuntimeError(f"rms_norm_quantize: residual must have x's shape {tuple(x.shape)}, "
                                f"got {tuple(residual.shape)}")
         r2 = _bf16_rows(residual, "rms_norm_quantize: residual")
-        h = torch.empty((M, H), dtype=torch.bfloat16, device=x.device)
+        h = _new(M, H, torch.bfloat16, x.device)
     w, wdt = _norm_weight(weight, H, "rms_norm_quantize")
     q = s = y = None
     if quantize:
-        q = torch.empty((M, H), dtype=torch.float8_e4m3fn, device=x.device)
+        q = _new(M, H, torch.float8_e4m3fn, x.device)
         s = empty_act_scales(M, H // 128, x.device)
     else:
-        y = torch.empty((M, H), dtype=torch.bfloat16, device=x.device)
-    rstd = torch.empty((M,), dtype=torch.float32, device=x.device)
+        y = _new(M, H, torch.bfloat16, x.device)
+    rstd = torch.empty_strided((M,), (1,), dtype=torch.float32, device=x.device)
     with _DeviceGuard(x):
         L.check(L.load().ltxfp8_rms_norm_quantize(
             x2.data_ptr(), _ld(x2), _ptr(r2), 0 if r2 is None else _ld(r2), M, H, _ptr(w), wdt, eps, _ptr(h), _ptr(q),
@@ -668,17 +679,17 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, wei
         if tuple(d2.shape) != (M, H):
             raise RuntimeError(f"{name}: dh has {tuple(d2.shape)} values, dy {(M, H)}")
     w, wdt = _norm_weight(weight, H, name)
-    dx = torch.empty((M, H), dtype=torch.bfloat16, device=dy.device)
+    dx = _new(M, H, torch.bfloat16, dy.device)
     dw = ws = None
     n = 0
     with _DeviceGuard(dy):
         if w is not None:
-            dw = torch.empty((H,), dtype=weight.dtype, device=dy.device)
+            dw = torch.empty_strided((H,), (1,), dtype=weight.dtype, device=dy.device)
             ws, n = _workspace("ltxfp8_rms_norm_backward_workspace_bytes", (M, H), dy.device)
         L.check(L.load().ltxfp8_rms_norm_backward(
             dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), rstd.data_ptr(), _ptr(w), wdt, _ptr(d2),
             0 if d2 is None else _ld(d2), M, H, dx.data_ptr(), _ptr(dw), _ptr(ws), n, _stream(dy)))
-    return dx.view(dy.shape), dw
+    return (dx if dy.dim() == 2 else dx.view(dy.shape)), dw
 
 
 def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: torch.Tensor,
@@ -713,7 +724,7 @@ def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: 
     if residual is not None and (residual.dtype != torch.bfloat16 or tuple(residual.shape) != (M, N)):
         raise RuntimeError(f"{name}: residual must be bf16 [{M}, {N}], got {residual.dtype} {tuple(residual.shape)}")
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=a_q.device)
+        out = _new(M, N, torch.bfloat16, a_q.device)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N) or not out.is_contiguous():
         raise RuntimeError(f"{name}: out must be a contiguous bf16 [{M}, {N}] tensor")
     if M == 0:
@@ -722,7 +733,7 @@ def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: 
     with _DeviceGuard(a_q):
         ld = scale_layout(sfa, M, KB)
         n = gemm_workspace_bytes(M, N, K, a_q.device) if split_k else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=a_q.device) if n else None
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=a_q.device) if n else None
         L.check(L.load().ltxfp8_gemm_residual(
             a_q.data_ptr(), sfa.data_ptr(), ld, w_q.data_ptr(), sfb.data_ptr(), _ptr(bias), _ptr(r2),
             0 if r2 is None else _ld(r2), out.data_ptr(), M, N, K, act, _ptr(ws), n, _stream(a_q)))
@@ -742,8 +753,7 @@ def act_quantize_save(z: torch.Tensor, activation: str = "gelu_tanh"):
     M, N = z2.shape
     out = []
     for _ in range(2):
-        out += [torch.empty((M, N), dtype=torch.float8_e4m3fn, device=z.device),
-                empty_act_scales(M, N // 128, z.device)]
+        out += [_new(M, N, torch.float8_e4m3fn, z.device), empty_act_scales(M, N // 128, z.device)]
     yq, ys, zq, zs = out
     with _DeviceGuard(z):
         L.check(L.load().ltxfp8_act_quantize_save(z2.data_ptr(), _ld(z2), M, N, act, yq.data_ptr(), ys.data_ptr(),
@@ -767,15 +777,15 @@ def act_backward(dy: torch.Tensor, z_q: torch.Tensor, z_scales: torch.Tensor, ac
     q2, z_scales, zld = _code_rows(z_q, z_scales, f"{name}: z")
     if tuple(q2.shape) != (M, N):
         raise RuntimeError(f"{name}: the checkpoint has {tuple(q2.shape)} values, dy {(M, N)}")
-    dz = torch.empty((M, N), dtype=torch.bfloat16, device=dy.device)
+    dz = _new(M, N, torch.bfloat16, dy.device)
     dq = ds = db = ws = None
     n = 0
     if quantize:
-        dq = torch.empty((M, N), dtype=torch.float8_e4m3fn, device=dy.device)
+        dq = _new(M, N, torch.float8_e4m3fn, dy.device)
         ds = empty_act_scales(M, N // 128, dy.device)
     with _DeviceGuard(dy):
         if dbias:
-            db = torch.empty((N,), dtype=torch.float32, device=dy.device)
+            db = torch.empty_strided((N,), (1,), dtype=torch.float32, device=dy.device)
             ws, n = _workspace("ltxfp8_act_backward_workspace_bytes", (M, N), dy.device)
         L.check(L.load().ltxfp8_act_backward(dy2.data_ptr(), _ld(dy2), q2.data_ptr(), z_scales.data_ptr(), zld, M, N,
                                              act, dz.data_ptr(), _ptr(dq), _ptr(ds), align4(M), _ptr(db), _ptr(ws), n,
@@ -789,7 +799,7 @@ def _wgrad(name, g, x2, x_scales, x_ld, alpha, transposed):
     if x2.shape[0] != M:
         raise RuntimeError(f"{name}: g has {M} rows, x {x2.shape[0]}")
     K = x2.shape[1]
-    out = torch.empty((K, N) if transposed else (N, K), dtype=torch.bfloat16, device=g.device)
+    out = _new(K, N, torch.bfloat16, g.device) if transposed else _new(N, K, torch.bfloat16, g.device)
     with _DeviceGuard(g):
         ws, n = _workspace("ltxfp8_wgrad_workspace_bytes", (M, N, K), g.device)
         L.check(L.load().ltxfp8_wgrad(g2.data_ptr(), _ld(g2), x2.data_ptr(), _ld(x2), _ptr(x_scales), x_ld,
