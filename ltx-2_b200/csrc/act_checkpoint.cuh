@@ -86,78 +86,135 @@ struct ActBwdParams {
   const uint8_t* zq;
   const float* zs;
   int64_t zs_ld;
-  int groups;         // N / 128
-  __nv_bfloat16* dz;  // [M, N] or null
-  uint8_t* dzq;       // [M, N] or null
+  int groups;                    // N / 128
+  int col_groups, rows, passes;  // 1x128 groups of a column block, rows of a pass, passes over M
+  __nv_bfloat16* dz;             // [M, N] or null
+  uint8_t* dzq;                  // [M, N] or null
   float* dzs;
   int64_t dzs_ld;
   float* db_part;  // [gridDim.y, N] partial column sums, or null
 };
 
-// A block owns kG adjacent 1x128 groups (8 lanes each) and walks the rows with stride
-// gridDim.y * rows-per-pass, so the bias gradient of its columns stays in registers; the
-// partial sums of the gridDim.y row shares are added by col_sum_kernel in a fixed order.
-constexpr int kActBwdUnroll = 2;
+// Block (x, y) owns column block x and walks the passes y, y + gridDim.y, ... of `rows` rows
+// each, so the bias gradient of its columns stays in registers; the partial sums of the
+// gridDim.y row shares are added by col_sum_kernel in a fixed order.  8 lanes hold a group.
+//
+// HBM-bound (6 bytes a value); the loop's arithmetic (two exponential-unit instructions and
+// about 20 others a value) hides the loads only if many are in flight, so bulk copies bring
+// dy and the codes through a ring of shared-memory stages.  A stage is released by one
+// arrival per warp as soon as its values are in registers.
+enum ActStatus : unsigned int { kStActLoad = 0x41010001u, kStActFree = 0x41010002u, kStActDrain = 0x41010003u };
+constexpr int kActBwdMaxGroups = 32;  // 4096 columns = 256 threads x 16
+constexpr int kActBwdStages = 8;
+constexpr uint32_t kActBwdDyBytes = kActBwdMaxGroups * 256;                    // 8 KB a pass
+constexpr uint32_t kActBwdStageBytes = kActBwdDyBytes + kActBwdMaxGroups * 128;  // + 4 KB of codes
+constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 96 KB: two blocks an SM
 
-template <int kAct, int kG>
-__global__ void __launch_bounds__(256) act_backward_kernel(const ActBwdParams p) {
-  constexpr int kRows = 32 / kG;  // rows of one pass
-  __shared__ float db_rows[kRows][kG * 128];
-  const int t = threadIdx.x % (8 * kG), r = threadIdx.x / (8 * kG);
-  const int kb = blockIdx.x * kG + t / 8;
-  const bool col_ok = kb < p.groups;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kG * 128 + t * kRunLen;
+template <int kAct>
+__global__ void __launch_bounds__(256, 2) act_backward_kernel(const ActBwdParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kActBwdStages], freed[kActBwdStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kb0 = blockIdx.x * p.col_groups;
+  const int ngroups = min(p.col_groups, p.groups - kb0);  // of this block
+  const int runs = p.col_groups * 8;
+  const int r = threadIdx.x / runs, t = threadIdx.x - r * runs;
+  const int kb = kb0 + t / 8;
+  const bool mine = r < p.rows && t < ngroups * 8;
+  const int64_t col0 = static_cast<int64_t>(kb0) * 128, col = col0 + t * kRunLen;
+  const int npass = (p.passes - static_cast<int>(blockIdx.y) + static_cast<int>(gridDim.y) - 1) /
+                    static_cast<int>(gridDim.y);
+
+  // Warp 0: fetch pass j of this block, two copies a row (its dy, its codes), one row a lane.
+  auto load_pass = [&](int j) {
+    const int s = j % kActBwdStages;
+    const int64_t m0 = (blockIdx.y + static_cast<int64_t>(j) * gridDim.y) * p.rows;
+    const int rows = static_cast<int>(p.M - m0 < p.rows ? p.M - m0 : p.rows);
+    if (lane == 0) mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(rows * ngroups) * 384u);
+    __syncwarp();
+    if (lane < rows) {
+      uint8_t* st = ring + s * kActBwdStageBytes;
+      const int64_t m = m0 + lane;
+      bulk_load(&full[s], st + lane * p.col_groups * 256, p.dy + m * p.dy_ld + col0, ngroups * 256u);
+      bulk_load(&full[s], st + kActBwdDyBytes + lane * p.col_groups * 128, p.zq + m * p.N + col0, ngroups * 128u);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kActBwdStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&freed[s], 8);
+    }
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  if (warp == 0)
+    for (int j = 0; j < kActBwdStages && j < npass; ++j) load_pass(j);
+
   float2 db[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) db[j] = make_float2(0.0f, 0.0f);
-
-  for (int64_t m0 = static_cast<int64_t>(blockIdx.y) * (kRows * kActBwdUnroll); m0 < p.M;
-       m0 += static_cast<int64_t>(gridDim.y) * (kRows * kActBwdUnroll)) {
-    Run16 vy[kActBwdUnroll];
-    uint4 vz[kActBwdUnroll];
-    float sc[kActBwdUnroll];
-#pragma unroll
-    for (int u = 0; u < kActBwdUnroll; ++u) {
-      const int64_t m = m0 + u * kRows + r;
-      const bool ok = col_ok && m < p.M;
-      vy[u] = ok ? ld_run(p.dy + m * p.dy_ld + col) : zero_run();
-      vz[u] = ok ? *reinterpret_cast<const uint4*>(p.zq + m * p.N + col) : make_uint4(0, 0, 0, 0);
-      sc[u] = ok ? __ldg(p.zs + static_cast<int64_t>(kb) * p.zs_ld + m) : 0.0f;
+  for (int k = 0; k < 8; ++k) db[k] = make_float2(0.0f, 0.0f);
+  const int64_t step = static_cast<int64_t>(gridDim.y) * p.rows;
+  int64_t m = static_cast<int64_t>(blockIdx.y) * p.rows + r;
+  const float* zs = p.zs + static_cast<int64_t>(mine ? kb : 0) * p.zs_ld;
+  float sc_next = (mine && m < p.M) ? __ldg(zs + m) : 0.0f;
+  int j = 0;
+  for (; j < npass; ++j, m += step) {
+    const int s = j % kActBwdStages;
+    const uint32_t ph = (j / kActBwdStages) & 1u;
+    const bool in = mine && m < p.M;
+    const float sc = sc_next;
+    sc_next = (mine && m + step < p.M) ? __ldg(zs + m + step) : 0.0f;
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, kStActLoad))) break;
+    const uint8_t* st = ring + s * kActBwdStageBytes;
+    Run16 vy = zero_run();
+    uint4 vz = make_uint4(0, 0, 0, 0);
+    if (in) {
+      vy = ld_run(reinterpret_cast<const __nv_bfloat16*>(st) + threadIdx.x * kRunLen);
+      vz = *reinterpret_cast<const uint4*>(st + kActBwdDyBytes + threadIdx.x * kRunLen);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&freed[s]);
+    float2 d[8], z[8];
+    run_to_f2(vy, d);
+    codes16_to_f2(vz, z);
+    const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-    for (int u = 0; u < kActBwdUnroll; ++u) {
-      const int64_t m = m0 + u * kRows + r;
-      const bool ok = col_ok && m < p.M;
-      float2 d[8], z[8];
-      run_to_f2(vy[u], d);
-      codes16_to_f2(vz[u], z);
-      const float2 s2 = make_float2(sc[u], sc[u]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        d[j] = __fmul2_rn(d[j], act_grad<kAct>(__fmul2_rn(z[j], s2)));
-        db[j] = __fadd2_rn(db[j], d[j]);
+    for (int k = 0; k < 8; ++k) {
+      d[k] = __fmul2_rn(d[k], act_grad<kAct>(__fmul2_rn(z[k], s2)));
+      db[k] = __fadd2_rn(db[k], d[k]);
+    }
+    if (p.dz != nullptr && in) st_run(p.dz + m * p.N + col, f2_to_run(d));
+    if (p.dzq != nullptr) {
+      float inv;
+      const uint4 c = quant_run16(d, inv);
+      if (in) {
+        *reinterpret_cast<uint4*>(p.dzq + m * p.N + col) = c;
+        if ((t & 7) == 0) p.dzs[static_cast<int64_t>(kb) * p.dzs_ld + m] = inv;
       }
-      if (p.dz != nullptr && ok) st_run(p.dz + m * p.N + col, f2_to_run(d));
-      if (p.dzq != nullptr) {
-        float inv;
-        const uint4 c = quant_run16(d, inv);
-        if (ok) {
-          *reinterpret_cast<uint4*>(p.dzq + m * p.N + col) = c;
-          if ((t & 7) == 0) p.dzs[static_cast<int64_t>(kb) * p.dzs_ld + m] = inv;
-        }
-      }
+    }
+    if (warp == 0 && j + kActBwdStages < npass) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&freed[s], ph, kStActFree))) break;
+      load_pass(j + kActBwdStages);
     }
   }
-  if (p.db_part == nullptr) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) *reinterpret_cast<float2*>(&db_rows[r][t * kRunLen + 2 * j]) = db[j];
+  if (j < npass && warp == 0) {
+    // A wait gave up: let the copies already issued land before the block exits.
+    const int issued = j + kActBwdStages < npass ? j + kActBwdStages : npass;
+    for (int i = j; i < issued; ++i) mbar_wait(&full[i % kActBwdStages], (i / kActBwdStages) & 1u, kStActDrain);
+  }
   __syncthreads();
-  for (int c = threadIdx.x; c < kG * 128; c += 256) {
-    float s = db_rows[0][c];
+  if (p.db_part == nullptr) return;
+  // The block's rows are added in row order, through the ring (every pass is consumed).
+  float* db_rows = reinterpret_cast<float*>(ring);
+  if (mine) {
 #pragma unroll
-    for (int i = 1; i < kRows; ++i) s += db_rows[i][c];
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * kG * 128 + c;
-    if (n < p.N) p.db_part[static_cast<int64_t>(blockIdx.y) * p.N + n] = s;
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<float2*>(db_rows + threadIdx.x * kRunLen + 2 * k) = db[k];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < ngroups * 128; c += 256) {
+    float s = db_rows[c];
+    for (int i = 1; i < p.rows; ++i) s += db_rows[i * p.col_groups * 128 + c];
+    p.db_part[static_cast<int64_t>(blockIdx.y) * p.N + col0 + c] = s;
   }
 }
 

@@ -94,6 +94,8 @@ struct DeviceInfo {
   int pair_clusters = 0;  // co-resident 2-CTA clusters of the pair kernel
   bool lora_ready = false;
   bool wgrad_ready[2] = {false, false};  // by x type: bf16, e4m3
+  bool norm_bwd_ready[6] = {};           // by (warps a row, runs a thread)
+  bool act_bwd_ready[2] = {};            // by activation
   float* static_scratch = nullptr;  // device address of g_gemm_static_scratch (ltxfp8_gemm_static_scratch)
 };
 
@@ -415,6 +417,28 @@ cudaError_t gated_launch(const DeviceInfo* d, cudaStream_t s, const __nv_bfloat1
 // Warps that share a row: one run of 16 values a thread up to H = 8192, two beyond.
 int norm_warps(int64_t H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
 int norm_block_rows(int64_t H) { return norm_warps(H) > 8 ? 1 : 8 / norm_warps(H); }
+
+// Shared memory of an SM for the backward's rings (228 KB less what a block reserves).
+constexpr uint32_t kNormRingBytes = 208 * 1024;
+
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, bool* ready, uint32_t bytes) {
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  if (*ready) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) *ready = true;
+  return e;
+}
+
+template <int kWarps, int kChunks>
+cudaError_t norm_bwd_launch(DeviceInfo* d, const NormBwdParams& p, unsigned grid, uint32_t smem, cudaStream_t s) {
+  constexpr int kIdx = kWarps == 1 ? 0 : kWarps == 2 ? 1 : kWarps == 4 ? 2 : kWarps == 8 ? 3 : kChunks == 1 ? 4 : 5;
+  auto kern = rms_norm_bwd_kernel<kWarps, kChunks>;
+  cudaError_t e = allow_smem(kern, &d->norm_bwd_ready[kIdx], kNormRingBytes / (kWarps > 8 ? 1 : 2));
+  if (e != cudaSuccess) return e;
+  kern<<<grid, norm_threads<kWarps>, smem, s>>>(p);
+  return cudaGetLastError();
+}
 
 template <int kWarps, int kChunks>
 void norm_fwd_launch(const NormFwdParams& p, unsigned grid, cudaStream_t s) {
@@ -1294,11 +1318,14 @@ int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, 
   return LTXFP8_OK;
 }
 
-// Blocks of the norm's backward: each SM's share of resident blocks, at most one per row group.
+// Blocks of the norm's backward: what is resident at once (two 256-thread blocks an SM, one
+// of 512 threads), at most one per row group.
+static int norm_bwd_per_sm(int64_t H) { return norm_warps(H) > 8 ? 1 : 2; }
+
 static int64_t norm_bwd_blocks(int sms, int64_t M, int64_t H) {
   const int rows = norm_block_rows(H);
   const int64_t groups = (M + rows - 1) / rows;
-  const int64_t cap = static_cast<int64_t>(sms) * (norm_warps(H) > 8 ? 2 : 4);
+  const int64_t cap = static_cast<int64_t>(sms) * norm_bwd_per_sm(H);
   return groups < cap ? groups : cap;
 }
 
@@ -1359,20 +1386,28 @@ int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64
   p.w_f32 = weight_dtype == LTXFP8_DTYPE_F32;
   p.dx = static_cast<__nv_bfloat16*>(dx);
   p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
+  // Ring stages: as many as fit the block's share of an SM's shared memory (at least two:
+  // the widest row with three inputs takes 96 KB a stage).
+  const int rows = norm_block_rows(H);
+  const uint32_t stage = static_cast<uint32_t>(rows) * (dh ? 3u : 2u) * static_cast<uint32_t>(H) * 2u;
+  int stages = static_cast<int>(kNormRingBytes / norm_bwd_per_sm(H) / stage);
+  if (stages > kNormMaxStages) stages = kNormMaxStages;
+  p.stages = stages;
+  // The row groups' gain gradients are joined in the same memory.
+  uint32_t smem = stage * static_cast<uint32_t>(stages);
+  if (rows > 1 && smem < 16384u) smem = 16384u;
   const unsigned grid = static_cast<unsigned>(blocks);
+  cudaError_t e;
   switch (norm_warps(H)) {
-    case 1: rms_norm_bwd_kernel<1, 1><<<grid, 256, 0, s>>>(p); break;
-    case 2: rms_norm_bwd_kernel<2, 1><<<grid, 256, 0, s>>>(p); break;
-    case 4: rms_norm_bwd_kernel<4, 1><<<grid, 256, 0, s>>>(p); break;
-    case 8: rms_norm_bwd_kernel<8, 1><<<grid, 256, 0, s>>>(p); break;
-    default:
-      if (H <= 8192) rms_norm_bwd_kernel<16, 1><<<grid, 512, 0, s>>>(p);
-      else rms_norm_bwd_kernel<16, 2><<<grid, 512, 0, s>>>(p);
+    case 1: e = norm_bwd_launch<1, 1>(d, p, grid, smem, s); break;
+    case 2: e = norm_bwd_launch<2, 1>(d, p, grid, smem, s); break;
+    case 4: e = norm_bwd_launch<4, 1>(d, p, grid, smem, s); break;
+    case 8: e = norm_bwd_launch<8, 1>(d, p, grid, smem, s); break;
+    default: e = H <= 8192 ? norm_bwd_launch<16, 1>(d, p, grid, smem, s) : norm_bwd_launch<16, 2>(d, p, grid, smem, s);
   }
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward launch");
   if (dweight) {
-    col_sum_kernel<<<static_cast<unsigned>((H + 31) / 32), 256, 0, s>>>(p.dw_part, static_cast<int>(blocks),
+    col_sum_kernel<<<static_cast<unsigned>((H + 31) / 32), kColSumWarps * 32, 0, s>>>(p.dw_part, static_cast<int>(blocks),
                                                                         static_cast<int>(H), dweight,
                                                                         weight_dtype == LTXFP8_DTYPE_F32);
     e = cudaGetLastError();
@@ -1436,17 +1471,22 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
   return LTXFP8_OK;
 }
 
-// Row shares of the activation's backward: enough blocks for several per SM.
-static dim3 act_bwd_grid(int sms, int64_t M, int64_t N) {
+// Blocks of the activation's backward: column blocks of up to 4096 columns, evenly divided,
+// times row shares that make up what is resident at once (two blocks an SM).
+struct ActBwdPlan {
+  int col_groups, col_blocks, rows, passes, shares;
+};
+
+static ActBwdPlan act_bwd_plan(int sms, int64_t M, int64_t N) {
+  ActBwdPlan a;
   const int64_t groups = N / 128;
-  const int kg = groups >= 4 ? 4 : 1;
-  const int64_t gx = (groups + kg - 1) / kg;
-  const int64_t passes = (M + 32 / kg * kActBwdUnroll - 1) / (32 / kg * kActBwdUnroll);
-  int64_t gy = (static_cast<int64_t>(sms) * 8 + gx - 1) / gx;
-  if (gy > passes) gy = passes;
-  if (gy > 65535) gy = 65535;
-  if (gy < 1) gy = 1;
-  return dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+  a.col_blocks = static_cast<int>((groups + kActBwdMaxGroups - 1) / kActBwdMaxGroups);
+  a.col_groups = static_cast<int>((groups + a.col_blocks - 1) / a.col_blocks);
+  a.rows = kActBwdMaxGroups / a.col_groups;
+  a.passes = static_cast<int>((M + a.rows - 1) / a.rows);
+  const int64_t want = (2 * static_cast<int64_t>(sms)) / a.col_blocks;
+  a.shares = static_cast<int>(want < 1 ? 1 : want < a.passes ? want : a.passes);
+  return a;
 }
 
 int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
@@ -1457,7 +1497,7 @@ int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
   DeviceInfo* d;
   rc = device_info(&d);
   if (rc) return rc;
-  *bytes = static_cast<size_t>(act_bwd_grid(d->sms, M, N).y) * static_cast<size_t>(N) * 4u;
+  *bytes = static_cast<size_t>(act_bwd_plan(d->sms, M, N).shares) * static_cast<size_t>(N) * 4u;
   return LTXFP8_OK;
 }
 
@@ -1483,9 +1523,9 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   DeviceInfo* d;
   rc = device_info(&d);
   if (rc) return rc;
-  const dim3 grid = act_bwd_grid(d->sms, M, N);
+  const ActBwdPlan pl = act_bwd_plan(d->sms, M, N);
   if (dbias) {
-    if (!workspace || workspace_bytes < static_cast<size_t>(grid.y) * static_cast<size_t>(N) * 4u)
+    if (!workspace || workspace_bytes < static_cast<size_t>(pl.shares) * static_cast<size_t>(N) * 4u)
       return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the workspace is missing or too small", name);
     if (!aligned(workspace, 16) || !aligned(dbias, 4))
       return fail(LTXFP8_ERR_MISALIGNED, "%s: workspace must be 16-byte, dbias 4-byte aligned", name);
@@ -1499,23 +1539,24 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   p.zs = zs;
   p.zs_ld = zs_ld;
   p.groups = static_cast<int>(N / 128);
+  p.col_groups = pl.col_groups;
+  p.rows = pl.rows;
+  p.passes = pl.passes;
   p.dz = static_cast<__nv_bfloat16*>(dz);
   p.dzq = static_cast<uint8_t*>(dzq);
   p.dzs = dzs;
   p.dzs_ld = dzs_ld;
   p.db_part = dbias ? static_cast<float*>(workspace) : nullptr;
+  const dim3 grid(static_cast<unsigned>(pl.col_blocks), static_cast<unsigned>(pl.shares));
   const bool gelu = activation == LTXFP8_ACT_GELU_TANH;
-  if (N >= 512) {
-    if (gelu) act_backward_kernel<kActGeluTanh, 4><<<grid, 256, 0, s>>>(p);
-    else act_backward_kernel<kActSilu, 4><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (gelu) act_backward_kernel<kActGeluTanh, 1><<<grid, 256, 0, s>>>(p);
-    else act_backward_kernel<kActSilu, 1><<<grid, 256, 0, s>>>(p);
-  }
-  cudaError_t e = cudaGetLastError();
+  auto kern = gelu ? act_backward_kernel<kActGeluTanh> : act_backward_kernel<kActSilu>;
+  cudaError_t e = allow_smem(kern, &d->act_bwd_ready[gelu], kActBwdSmemBytes);
+  if (e != cudaSuccess) return cuda_fail(e, "act_backward smem");
+  kern<<<grid, 256, kActBwdSmemBytes, s>>>(p);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "act_backward launch");
   if (dbias) {
-    col_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), 256, 0, s>>>(p.db_part, static_cast<int>(grid.y),
+    col_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), kColSumWarps * 32, 0, s>>>(p.db_part, pl.shares,
                                                                         static_cast<int>(N), dbias, true);
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "act_backward sum launch");

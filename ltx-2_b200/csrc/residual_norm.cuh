@@ -204,19 +204,57 @@ struct NormBwdParams {
   bool w_f32;
   __nv_bfloat16* dx;  // [M, H]
   float* dw_part;     // [gridDim.x, H] partial sums over the block's rows, or null
+  int stages;         // of the shared-memory ring, at most kNormMaxStages
 };
 
 // A persistent grid: block b takes the row groups b, b + gridDim.x, ... and keeps the
 // gain gradient of its rows in registers; the blocks' partial sums are added by
 // col_sum_kernel in block order, so the result does not depend on scheduling.
+//
+// HBM-bound (8 bytes a value with dh), but a row is a reduction, a barrier and a second
+// pass: with register loads too few bytes are in flight behind them.  So bulk copies
+// bring the rows through a ring of `stages` shared-memory stages; a stage is free again at
+// the row's own barrier, when every thread has its values in registers.
+enum NormStatus : unsigned int { kStNormLoad = 0x4E010001u, kStNormDrain = 0x4E010002u };
+constexpr int kNormMaxStages = 8;
+
 template <int kWarps, int kChunks>
 __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(const NormBwdParams p) {
   constexpr int kRows = norm_threads<kWarps> / (32 * kWarps);
   __shared__ float red[2][norm_threads<kWarps> / 32];
-  __shared__ float dw_rows[kRows > 1 ? kRows * kWarps * 32 * kChunks * kRunLen : 1];
+  __shared__ uint64_t full[kNormMaxStages];
+  extern __shared__ __align__(128) uint8_t ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = (warp % kWarps) * 32 + lane;
   const float inv_h = 1.0f / static_cast<float>(p.H);
+  const int inputs = p.dh != nullptr ? 3 : 2;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.H) * 2u;
+  const uint32_t stage_bytes = row_bytes * kRows * inputs;
+  const int64_t row_groups = (p.M + kRows - 1) / kRows;
+  const int passes = static_cast<int>((row_groups - blockIdx.x + gridDim.x - 1) / gridDim.x);
+
+  // Warp 0: fetch the rows of pass j, one copy a lane (row r of input i at (r * inputs + i)).
+  auto load_pass = [&](int j) {
+    const int64_t r0 = (blockIdx.x + static_cast<int64_t>(j) * gridDim.x) * kRows;
+    const int rows = static_cast<int>(p.M - r0 < kRows ? p.M - r0 : kRows);
+    uint64_t* bar = &full[j % p.stages];
+    if (lane == 0) mbar_arrive_expect_tx(bar, row_bytes * rows * inputs);
+    __syncwarp();
+    if (lane < rows * inputs) {
+      const int r = lane / inputs, i = lane - r * inputs;
+      const __nv_bfloat16* src = i == 0   ? p.dy + (r0 + r) * p.dy_ld
+                                 : i == 1 ? p.h + (r0 + r) * p.h_ld
+                                          : p.dh + (r0 + r) * p.dh_ld;
+      bulk_load(bar, ring + (j % p.stages) * stage_bytes + lane * row_bytes, src, row_bytes);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  if (warp == 0)
+    for (int j = 0; j < p.stages && j < passes; ++j) load_pass(j);
 
   float2 dw[kChunks][8];
 #pragma unroll
@@ -224,40 +262,50 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = make_float2(0.0f, 0.0f);
 
-  int phase = 0;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < p.M;
-       r0 += static_cast<int64_t>(gridDim.x) * kRows, phase ^= 1) {
-    const int64_t row = r0 + warp / kWarps;
+  const int64_t row_step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp / kWarps;
+  float rstd_next = row < p.M ? __ldg(p.rstd + row) : 0.0f;
+  bool ok = true;
+  int j = 0;
+  for (; j < passes; ++j, row += row_step) {
     const bool row_ok = row < p.M;
-    const float rstd = row_ok ? __ldg(p.rstd + row) : 0.0f;
+    const float rstd = rstd_next;
+    rstd_next = row + row_step < p.M ? __ldg(p.rstd + row + row_step) : 0.0f;
+    ok = mbar_wait(&full[j % p.stages], (j / p.stages) & 1u, kStNormLoad);
+    const uint8_t* src = ring + (j % p.stages) * stage_bytes + (warp / kWarps) * inputs * row_bytes;
     Run16 vy[kChunks], vh[kChunks], vd[kChunks];
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (i * kWarps * 32 + t) * kRunLen;
-      const bool ok = row_ok && col < p.H;
-      vy[i] = ok ? ld_run(p.dy + row * p.dy_ld + col) : zero_run();
-      vh[i] = ok ? ld_run(p.h + row * p.h_ld + col) : zero_run();
-      vd[i] = (ok && p.dh != nullptr) ? ld_run(p.dh + row * p.dh_ld + col) : zero_run();
-    }
     float acc = 0.0f;
     const float2 r2 = make_float2(rstd, rstd);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int col = (i * kWarps * 32 + t) * kRunLen;
+      const bool in = row_ok && col < p.H;
+      const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(src) + col;
+      vy[i] = in ? ld_run(v) : zero_run();
+      vh[i] = in ? ld_run(v + p.H) : zero_run();
+      vd[i] = (in && inputs == 3) ? ld_run(v + 2 * p.H) : zero_run();
       float2 y[8], x[8], w[8], s = make_float2(0.0f, 0.0f);
       run_to_f2(vy[i], y);
       run_to_f2(vh[i], x);
       ld_gain(p.w, p.w_f32, col < p.H ? col : 0, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 yx = __fmul2_rn(y[j], __fmul2_rn(x[j], r2));  // dy * xhat
-        dw[i][j] = __fadd2_rn(dw[i][j], yx);
-        s = __ffma2_rn(yx, w[j], s);
+      for (int k = 0; k < 8; ++k) {
+        const float2 yx = __fmul2_rn(y[k], __fmul2_rn(x[k], r2));  // dy * xhat
+        dw[i][k] = __fadd2_rn(dw[i][k], yx);
+        s = __ffma2_rn(yx, w[k], s);
       }
       acc += s.x + s.y;
     }
-    const float c = row_sum<kWarps>(acc, red[phase], warp) * inv_h;
-    const float2 c2 = make_float2(-c, -c);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (lane == 0) red[j & 1][warp] = acc;
+    if (!__syncthreads_and(ok)) break;
+    if (warp == 0 && j + p.stages < passes) load_pass(j + p.stages);
+    float c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) c += red[j & 1][warp / kWarps * kWarps + i];
+    c *= -inv_h;
+    const float2 c2 = make_float2(c, c);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int col = (i * kWarps * 32 + t) * kRunLen;
@@ -267,10 +315,16 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
       run_to_f2(vd[i], d);
       ld_gain(p.w, p.w_f32, col < p.H ? col : 0, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        d[j] = __ffma2_rn(r2, __ffma2_rn(__fmul2_rn(x[j], r2), c2, __fmul2_rn(y[j], w[j])), d[j]);
+      for (int k = 0; k < 8; ++k)
+        d[k] = __ffma2_rn(r2, __ffma2_rn(__fmul2_rn(x[k], r2), c2, __fmul2_rn(y[k], w[k])), d[k]);
       if (row_ok && col < p.H) st_run(p.dx + row * p.H + col, f2_to_run(d));
     }
+  }
+  if (j < passes) {
+    // A wait gave up: let the copies already issued land before the block exits.
+    const int issued = j + p.stages < passes ? j + p.stages : passes;
+    for (int i = j; i < issued; ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u, kStNormDrain);
+    return;
   }
   if (p.dw_part == nullptr) return;
   float* part = p.dw_part + static_cast<int64_t>(blockIdx.x) * p.H;
@@ -281,19 +335,21 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
       if (col < p.H) {
         float4* dst = reinterpret_cast<float4*>(part + col);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          dst[j] = make_float4(dw[i][2 * j].x, dw[i][2 * j].y, dw[i][2 * j + 1].x, dw[i][2 * j + 1].y);
+        for (int k = 0; k < 4; ++k)
+          dst[k] = make_float4(dw[i][2 * k].x, dw[i][2 * k].y, dw[i][2 * k + 1].x, dw[i][2 * k + 1].y);
       }
     }
   } else {
-    // The block's row groups are added in row order.
+    // The block's row groups are added in row order, through the ring (all passes are consumed).
     constexpr int kRowLen = kWarps * 32 * kChunks * kRunLen;
+    float* dw_rows = reinterpret_cast<float*>(ring);
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<float2*>(dw_rows + (warp / kWarps) * kRowLen + (i * kWarps * 32 + t) * kRunLen + 2 * j) =
-            dw[i][j];
+      for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<float2*>(dw_rows + (warp / kWarps) * kRowLen + (i * kWarps * 32 + t) * kRunLen + 2 * k) =
+            dw[i][k];
     __syncthreads();
     for (int col = threadIdx.x; col < p.H; col += norm_threads<kWarps>) {
       float s = dw_rows[col];
@@ -305,22 +361,23 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
 }
 
 // out[n] = sum over p of part[p, n], in the type of `out` (fp32 or bf16): a block sums 32
-// columns, its 8 warps every eighth partial row each, in a fixed order.
-__global__ void __launch_bounds__(256) col_sum_kernel(const float* __restrict__ part, int parts, int N, void* out,
+// columns, its kColSumWarps warps every kColSumWarps-th partial row each, in a fixed order.
+constexpr int kColSumWarps = 32;
+__global__ void __launch_bounds__(kColSumWarps * 32) col_sum_kernel(const float* __restrict__ part, int parts, int N, void* out,
                                                       bool out_f32) {
-  __shared__ float red[8][32];
+  __shared__ float red[kColSumWarps][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (n < N) {
 #pragma unroll 8
-    for (int i = warp; i < parts; i += 8) s += part[static_cast<int64_t>(i) * N + n];
+    for (int i = warp; i < parts; i += kColSumWarps) s += part[static_cast<int64_t>(i) * N + n];
   }
   red[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && n < N) {
 #pragma unroll
-    for (int w = 1; w < 8; ++w) s += red[w][lane];
+    for (int w = 1; w < kColSumWarps; ++w) s += red[w][lane];
     if (out_f32)
       static_cast<float*>(out)[n] = s;
     else
