@@ -43,7 +43,7 @@ constexpr int kActSaveUnroll = 2;
 constexpr int kActSaveGroups = 32 * kActSaveUnroll;  // 1x128 groups of a 256-thread block
 
 template <int kAct>
-__global__ void __launch_bounds__(256) act_quantize_save_kernel(const ActSaveParams p) {
+__global__ void __launch_bounds__(256, 6) act_quantize_save_kernel(const ActSaveParams p) {
   const int64_t g0 = static_cast<int64_t>(blockIdx.x) * kActSaveGroups;
   const int64_t row0 = g0 / p.groups;
   const uint32_t kb0 = static_cast<uint32_t>(g0 - row0 * p.groups);
@@ -105,13 +105,13 @@ struct ActBwdParams {
 // arrival per warp as soon as its values are in registers.
 enum ActStatus : unsigned int { kStActLoad = 0x41010001u, kStActFree = 0x41010002u, kStActDrain = 0x41010003u };
 constexpr int kActBwdMaxGroups = 32;  // 4096 columns = 256 threads x 16
-constexpr int kActBwdStages = 8;
+constexpr int kActBwdStages = 6;
 constexpr uint32_t kActBwdDyBytes = kActBwdMaxGroups * 256;                    // 8 KB a pass
 constexpr uint32_t kActBwdStageBytes = kActBwdDyBytes + kActBwdMaxGroups * 128;  // + 4 KB of codes
-constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 96 KB: two blocks an SM
+constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 72 KB: three blocks an SM
 
 template <int kAct>
-__global__ void __launch_bounds__(256, 2) act_backward_kernel(const ActBwdParams p) {
+__global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[kActBwdStages], freed[kActBwdStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

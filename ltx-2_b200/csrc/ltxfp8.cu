@@ -1386,12 +1386,13 @@ int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64
   p.w_f32 = weight_dtype == LTXFP8_DTYPE_F32;
   p.dx = static_cast<__nv_bfloat16*>(dx);
   p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
-  // Ring stages: as many as fit the block's share of an SM's shared memory (at least two:
-  // the widest row with three inputs takes 96 KB a stage).
+  // Ring stages: 48 KB a block (enough in flight; 96 KB measured 3 % slower at H = 4096), but
+  // at least two (the widest row with three inputs takes 96 KB a stage).
   const int rows = norm_block_rows(H);
   const uint32_t stage = static_cast<uint32_t>(rows) * (dh ? 3u : 2u) * static_cast<uint32_t>(H) * 2u;
-  int stages = static_cast<int>(kNormRingBytes / norm_bwd_per_sm(H) / stage);
+  int stages = static_cast<int>(48u * 1024u / stage);
   if (stages > kNormMaxStages) stages = kNormMaxStages;
+  if (stages < 2) stages = 2;
   p.stages = stages;
   // The row groups' gain gradients are joined in the same memory.
   uint32_t smem = stage * static_cast<uint32_t>(stages);
@@ -1472,7 +1473,7 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
 }
 
 // Blocks of the activation's backward: column blocks of up to 4096 columns, evenly divided,
-// times row shares that make up what is resident at once (two blocks an SM).
+// times row shares that make up what is resident at once (three blocks an SM).
 struct ActBwdPlan {
   int col_groups, col_blocks, rows, passes, shares;
 };
@@ -1484,7 +1485,7 @@ static ActBwdPlan act_bwd_plan(int sms, int64_t M, int64_t N) {
   a.col_groups = static_cast<int>((groups + a.col_blocks - 1) / a.col_blocks);
   a.rows = kActBwdMaxGroups / a.col_groups;
   a.passes = static_cast<int>((M + a.rows - 1) / a.rows);
-  const int64_t want = (2 * static_cast<int64_t>(sms)) / a.col_blocks;
+  const int64_t want = (3 * static_cast<int64_t>(sms)) / a.col_blocks;
   a.shares = static_cast<int>(want < 1 ? 1 : want < a.passes ? want : a.passes);
   return a;
 }
