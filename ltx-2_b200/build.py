@@ -5,6 +5,11 @@ status word and the kernels share one module.  The library links the CUDA
 runtime statically and reaches the driver's tensor-map encoder through
 ``cudaGetDriverEntryPointByVersion``; it needs no torch headers.
 
+The tensor-level calls of the residual-path and training operators
+(``csrc/torch_binding.cpp``) are a second library, ``lib/_ltxfp8_torch.so``: host code
+only, compiled with g++ against torch's headers and linked to the first by a
+relative path.
+
 Usage:  python ltx-2_b200/build.py [--force] [--verbose]
 """
 from __future__ import annotations
@@ -18,6 +23,7 @@ REPO = os.path.dirname(HERE)
 SRC_DIR = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libltxfp8.so")
+BINDING_PATH = os.path.join(LIB_DIR, "_ltxfp8_torch.so")
 INCLUDE = os.path.join(REPO, "include")
 
 NVCC_FLAGS = [
@@ -34,15 +40,43 @@ def _sources():
     return files
 
 
-def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _stale(target, sources) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(f) > t for f in _sources())
+    t = os.path.getmtime(target)
+    return any(os.path.getmtime(f) > t for f in sources)
+
+
+def needs_build() -> bool:
+    return _stale(LIB_PATH, _sources())
+
+
+def build_binding(force: bool = False) -> str:
+    src = os.path.join(SRC_DIR, "torch_binding.cpp")
+    if not force and not _stale(BINDING_PATH, [src, os.path.join(INCLUDE, "ltxfp8.h")]):
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    tmp = os.path.join(LIB_DIR, "_ltxfp8_torch.tmp.so")
+    subprocess.check_call([
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-I" + INCLUDE, "-isystem", os.path.join(root, "include"),
+        "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+        "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
+        src, "-o", tmp, "-L" + LIB_DIR, "-l:libltxfp8.so", "-L" + os.path.join(root, "lib"),
+        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
+        build_binding()
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
     nvcc = os.environ.get("NVCC", "nvcc")
@@ -54,6 +88,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd))
     subprocess.check_call(cmd)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
+    build_binding(force)
     return LIB_PATH
 
 

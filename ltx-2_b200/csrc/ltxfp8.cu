@@ -1597,6 +1597,13 @@ struct WgradPlan {
 };
 
 static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
+  // The plan of the last shape on this thread: a call asks for it twice (workspace, launch).
+  static thread_local struct {
+    int sms;
+    int64_t M, N, K;
+    WgradPlan plan;
+  } last{};
+  if (last.sms == sms && last.M == M && last.N == N && last.K == K) return last.plan;
   WgradPlan best{};
   double best_cost = 0.0;
   const int64_t stages = (M + kWgStageM - 1) / kWgStageM, k_tiles = (K + kWgTileK - 1) / kWgTileK;
@@ -1619,6 +1626,11 @@ static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
       }
     }
   }
+  last.sms = sms;
+  last.M = M;
+  last.N = N;
+  last.K = K;
+  last.plan = best;
   return best;
 }
 

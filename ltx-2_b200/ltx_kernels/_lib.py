@@ -11,6 +11,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libltxfp8.so")
+BINDING_PATH = os.path.join(os.path.dirname(_HERE), "lib", "_ltxfp8_torch.so")
 
 # Error codes of include/ltxfp8.h
 OK = 0
@@ -145,6 +146,32 @@ def load(path: str | None = None):
                 fn.argtypes = args
             _lib = L
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """Load (once) and return the compiled tensor-level calls (csrc/torch_binding.cpp)."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    load()
+    with _lock:
+        if _binding is None:
+            if not os.path.exists(BINDING_PATH):
+                raise ImportError(
+                    f"{BINDING_PATH} is missing: build it first (python ltx-2_b200/build.py, or "
+                    "__graft_entry__.build())")
+            import importlib.util
+
+            import torch  # noqa: F401  (its libraries must be loaded first)
+            spec = importlib.util.spec_from_file_location("_ltxfp8_torch", BINDING_PATH)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            mod.set_check(check)
+            _binding = mod
+    return _binding
 
 
 def check(rc: int) -> None:

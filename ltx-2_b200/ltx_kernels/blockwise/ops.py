@@ -541,83 +541,11 @@ def lora_a(x: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------- residual path and training
-_ACTIVATIONS = {None: L.ACT_NONE, "gelu_tanh": L.ACT_GELU_TANH, "silu": L.ACT_SILU}
-
-
-def _activation(name: str, activation, allow_none: bool) -> int:
-    if activation not in _ACTIVATIONS or (activation is None and not allow_none):
-        kinds = "None, 'gelu_tanh' or 'silu'" if allow_none else "'gelu_tanh' or 'silu'"
-        raise RuntimeError(f"{name}: activation must be {kinds}, got {activation!r}")
-    return _ACTIVATIONS[activation]
-
-
-def _bf16_rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """bf16 [..., K] as an [M, K] matrix with 16-byte aligned rows (a copy only where it has none)."""
-    if x.dtype != torch.bfloat16:
-        raise RuntimeError(f"{name}: expected bf16, got {x.dtype}")
-    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0 and x.shape[1] % 8 == 0 and x.shape[1]:
-        return x
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise RuntimeError(f"{name}: expected a [..., K] tensor, got shape {tuple(x.shape)}")
-    x2 = x.reshape(-1, x.shape[-1])
-    M, K = x2.shape
-    if M > 0 and (x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (x2.stride(0) % 8 or x2.stride(0) < K))):
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2
-
-
-def _new(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
-    """torch.empty((M, N)): the strided form parses its arguments faster (1.5 against 2.3 us)."""
-    return torch.empty_strided((M, N), (N, 1), dtype=dtype, device=device)
-
-
-def _ld(x2: torch.Tensor) -> int:
-    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-
-
-def _code_rows(q: torch.Tensor, scales: torch.Tensor, name: str) -> Tuple[torch.Tensor, torch.Tensor, int]:
-    """e4m3 codes [..., K] as a contiguous aligned [M, K] matrix, their scales, and the scales' stride."""
-    if q.dtype != torch.float8_e4m3fn:
-        raise RuntimeError(f"{name}: codes must be float8_e4m3fn, got {q.dtype}")
-    if q.dim() < 1 or q.shape[-1] == 0 or q.shape[-1] % 128:
-        raise RuntimeError(f"{name}: expected [..., K] codes with K a positive multiple of 128, got {tuple(q.shape)}")
-    q2 = q if q.dim() == 2 and q.is_contiguous() else q.reshape(-1, q.shape[-1]).contiguous()
-    if q2.data_ptr() % 16:
-        q2 = q2.clone()
-    M, K = q2.shape
-    return q2, scales, (scale_layout(scales, M, K // 128) if M else 1)
-
-
-def _norm_weight(weight: Optional[torch.Tensor], H: int, name: str):
-    """(contiguous aligned weight or None, its dtype code)."""
-    if weight is None:
-        return None, L.DTYPE_F32
-    dt = {torch.float32: L.DTYPE_F32, torch.bfloat16: L.DTYPE_BF16}.get(weight.dtype)
-    if dt is None or tuple(weight.shape) != (H,):
-        raise RuntimeError(f"{name}: weight must be fp32 or bf16 [{H}], got {weight.dtype} {tuple(weight.shape)}")
-    weight = weight.contiguous()
-    return (weight.clone() if weight.data_ptr() % 16 else weight), dt
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-_TRAIN_WS_CACHE: dict = {}
-
-
-def _workspace(fn: str, dims: Tuple[int, ...], device) -> Tuple[Optional[torch.Tensor], int]:
-    """Scratch of the library's ``fn`` for these dimensions, from the caching allocator."""
-    key = (fn, device.index, dims)
-    n = _TRAIN_WS_CACHE.get(key)
-    if n is None:
-        import ctypes
-        b = ctypes.c_size_t(0)
-        L.check(getattr(L.load(), fn)(*dims, ctypes.byref(b)))
-        n = _TRAIN_WS_CACHE[key] = b.value
-    return (torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device) if n else None), n
-
-
+#
+# The checks, allocations and launches of these operators are compiled
+# (csrc/torch_binding.cpp): they are called per layer and step on few tokens as well, where
+# the host's time for a call counts.  Errors are the ones the other wrappers raise.  Rows may
+# be strided; a tensor without 16-byte aligned rows is copied first.
 def rms_norm_quantize(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                       residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6, quantize: bool = True):
     """RMS norm with the residual's addition and an 8-bit output.
@@ -628,31 +556,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``(codes [M, H], scales (M, H/128), h, rstd [M])``, or with ``quantize=False``
     ``(y bf16 [M, H], h, rstd)``; ``h`` and ``rstd`` are what :func:`rms_norm_backward`
     needs.  All-zero rows quantise to zero codes."""
-    _require_cuda("rms_norm_quantize", x, weight, residual)
-    x2 = _bf16_rows(x, "rms_norm_quantize: x")
-    M, H = x2.shape
-    r2 = h = None
-    if residual is not None:
-        if residual.shape != x.shape:
-            raise RuntimeError(f"rms_norm_quantize: residual must have x's shape {tuple(x.shape)}, "
-                               f"got {tuple(residual.shape)}")
-        r2 = _bf16_rows(residual, "rms_norm_quantize: residual")
-        h = _new(M, H, torch.bfloat16, x.device)
-    w, wdt = _norm_weight(weight, H, "rms_norm_quantize")
-    q = s = y = None
-    if quantize:
-        q = _new(M, H, torch.float8_e4m3fn, x.device)
-        s = empty_act_scales(M, H // 128, x.device)
-    else:
-        y = _new(M, H, torch.bfloat16, x.device)
-    rstd = torch.empty_strided((M,), (1,), dtype=torch.float32, device=x.device)
-    with _DeviceGuard(x):
-        L.check(L.load().ltxfp8_rms_norm_quantize(
-            x2.data_ptr(), _ld(x2), _ptr(r2), 0 if r2 is None else _ld(r2), M, H, _ptr(w), wdt, eps, _ptr(h), _ptr(q),
-            _ptr(s), align4(M), _ptr(y), rstd.data_ptr(), _stream(x)))
-    if h is None:
-        h = x2
-    return (q, s, h, rstd) if quantize else (y, h, rstd)
+    return L.binding().rms_norm_quantize(x, weight, residual, eps, quantize)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -664,32 +568,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, wei
     ``(dx, dweight)``: ``dx = rstd * (g - xhat * mean(g * xhat)) + dh`` with ``g = dy * weight``
     and ``xhat = h * rstd``, bf16 of dy's shape and the gradient of ``x`` and of the residual
     alike; ``dweight = sum(dy * xhat)`` in the weight's type (None without one)."""
-    name = "rms_norm_backward"
-    _require_cuda(name, dy, h, rstd, weight, dh)
-    dy2, h2 = _bf16_rows(dy, f"{name}: dy"), _bf16_rows(h, f"{name}: h")
-    M, H = dy2.shape
-    if tuple(h2.shape) != (M, H):
-        raise RuntimeError(f"{name}: h has {tuple(h2.shape)} values, dy {(M, H)}")
-    if rstd.dtype != torch.float32 or rstd.numel() != M:
-        raise RuntimeError(f"{name}: rstd must be fp32 [{M}]")
-    rstd = rstd.contiguous()
-    d2 = None
-    if dh is not None:
-        d2 = _bf16_rows(dh, f"{name}: dh")
-        if tuple(d2.shape) != (M, H):
-            raise RuntimeError(f"{name}: dh has {tuple(d2.shape)} values, dy {(M, H)}")
-    w, wdt = _norm_weight(weight, H, name)
-    dx = _new(M, H, torch.bfloat16, dy.device)
-    dw = ws = None
-    n = 0
-    with _DeviceGuard(dy):
-        if w is not None:
-            dw = torch.empty_strided((H,), (1,), dtype=weight.dtype, device=dy.device)
-            ws, n = _workspace("ltxfp8_rms_norm_backward_workspace_bytes", (M, H), dy.device)
-        L.check(L.load().ltxfp8_rms_norm_backward(
-            dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), rstd.data_ptr(), _ptr(w), wdt, _ptr(d2),
-            0 if d2 is None else _ld(d2), M, H, dx.data_ptr(), _ptr(dw), _ptr(ws), n, _stream(dy)))
-    return (dx if dy.dim() == 2 else dx.view(dy.shape)), dw
+    return L.binding().rms_norm_backward(dy, h, rstd, weight, dh)
 
 
 def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: torch.Tensor,
@@ -701,43 +580,7 @@ def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: 
 
     Operands as for :func:`gemm`; ``residual`` is bf16 [M, N] (rows may be strided),
     ``activation`` None, ``"gelu_tanh"`` or ``"silu"``.  ``out`` may be the residual itself."""
-    name = "gemm_residual"
-    _require_cuda(name, a_q, sfa, w_q, sfb, bias, residual, out)
-    act = _activation(name, activation, True)
-    if a_q.dim() != 2 or w_q.dim() != 2:
-        raise RuntimeError(f"{name} expects 2-D operands")
-    M, K = a_q.shape
-    N, K2 = w_q.shape
-    if K != K2:
-        raise RuntimeError(f"{name}: K mismatch ({K} vs {K2})")
-    if a_q.dtype != torch.float8_e4m3fn or w_q.dtype != torch.float8_e4m3fn:
-        raise RuntimeError(f"{name}: operands must be float8_e4m3fn")
-    if not a_q.is_contiguous() or not w_q.is_contiguous():
-        raise RuntimeError(f"{name}: operands must be contiguous (K-major)")
-    KB = K // 128
-    if sfb.dtype != torch.float32 or tuple(sfb.shape) != (N // 128, KB) or not sfb.is_contiguous():
-        raise RuntimeError(f"{name}: weight scales must be contiguous fp32 [{N // 128}, {KB}]")
-    if bias is not None:
-        if bias.dtype != torch.float32 or bias.numel() != N:
-            raise RuntimeError(f"{name}: bias must be fp32 [N]")
-        bias = bias.contiguous()
-    if residual is not None and (residual.dtype != torch.bfloat16 or tuple(residual.shape) != (M, N)):
-        raise RuntimeError(f"{name}: residual must be bf16 [{M}, {N}], got {residual.dtype} {tuple(residual.shape)}")
-    if out is None:
-        out = _new(M, N, torch.bfloat16, a_q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N) or not out.is_contiguous():
-        raise RuntimeError(f"{name}: out must be a contiguous bf16 [{M}, {N}] tensor")
-    if M == 0:
-        return out
-    r2 = None if residual is None else _bf16_rows(residual, f"{name}: residual")
-    with _DeviceGuard(a_q):
-        ld = scale_layout(sfa, M, KB)
-        n = gemm_workspace_bytes(M, N, K, a_q.device) if split_k else 0
-        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=a_q.device) if n else None
-        L.check(L.load().ltxfp8_gemm_residual(
-            a_q.data_ptr(), sfa.data_ptr(), ld, w_q.data_ptr(), sfb.data_ptr(), _ptr(bias), _ptr(r2),
-            0 if r2 is None else _ld(r2), out.data_ptr(), M, N, K, act, _ptr(ws), n, _stream(a_q)))
-    return out
+    return L.binding().gemm_residual(a_q, sfa, w_q, sfb, bias, residual, activation, out, split_k)
 
 
 def act_quantize_save(z: torch.Tensor, activation: str = "gelu_tanh"):
@@ -746,19 +589,7 @@ def act_quantize_save(z: torch.Tensor, activation: str = "gelu_tanh"):
     Returns ``(y_codes, y_scales, z_codes, z_scales)``: the 1x128 quantisation of ``act(z)``
     (``"gelu_tanh"`` or ``"silu"``), the next GEMM's operand, and that of ``z``, which is all
     that :func:`act_backward` needs.  Codes are [M, N], scales (M, N/128)."""
-    name = "act_quantize_save"
-    _require_cuda(name, z)
-    act = _activation(name, activation, False)
-    z2 = _bf16_rows(z, f"{name}: z")
-    M, N = z2.shape
-    out = []
-    for _ in range(2):
-        out += [_new(M, N, torch.float8_e4m3fn, z.device), empty_act_scales(M, N // 128, z.device)]
-    yq, ys, zq, zs = out
-    with _DeviceGuard(z):
-        L.check(L.load().ltxfp8_act_quantize_save(z2.data_ptr(), _ld(z2), M, N, act, yq.data_ptr(), ys.data_ptr(),
-                                                  align4(M), zq.data_ptr(), zs.data_ptr(), align4(M), _stream(z)))
-    return yq, ys, zq, zs
+    return L.binding().act_quantize_save(z, activation)
 
 
 def act_backward(dy: torch.Tensor, z_q: torch.Tensor, z_scales: torch.Tensor, activation: str = "gelu_tanh", *,
@@ -769,42 +600,7 @@ def act_backward(dy: torch.Tensor, z_q: torch.Tensor, z_scales: torch.Tensor, ac
     ``(dz, dz_codes, dz_scales, dbias)``: dz bf16 [M, N]; with ``quantize`` its 1x128
     quantisation too (the input-gradient GEMM's operand); with ``dbias`` its sum over rows,
     fp32 [N].  What was not asked for is None."""
-    name = "act_backward"
-    _require_cuda(name, dy, z_q, z_scales)
-    act = _activation(name, activation, False)
-    dy2 = _bf16_rows(dy, f"{name}: dy")
-    M, N = dy2.shape
-    q2, z_scales, zld = _code_rows(z_q, z_scales, f"{name}: z")
-    if tuple(q2.shape) != (M, N):
-        raise RuntimeError(f"{name}: the checkpoint has {tuple(q2.shape)} values, dy {(M, N)}")
-    dz = _new(M, N, torch.bfloat16, dy.device)
-    dq = ds = db = ws = None
-    n = 0
-    if quantize:
-        dq = _new(M, N, torch.float8_e4m3fn, dy.device)
-        ds = empty_act_scales(M, N // 128, dy.device)
-    with _DeviceGuard(dy):
-        if dbias:
-            db = torch.empty_strided((N,), (1,), dtype=torch.float32, device=dy.device)
-            ws, n = _workspace("ltxfp8_act_backward_workspace_bytes", (M, N), dy.device)
-        L.check(L.load().ltxfp8_act_backward(dy2.data_ptr(), _ld(dy2), q2.data_ptr(), z_scales.data_ptr(), zld, M, N,
-                                             act, dz.data_ptr(), _ptr(dq), _ptr(ds), align4(M), _ptr(db), _ptr(ws), n,
-                                             _stream(dy)))
-    return dz, dq, ds, db
-
-
-def _wgrad(name, g, x2, x_scales, x_ld, alpha, transposed):
-    g2 = _bf16_rows(g, f"{name}: g")
-    M, N = g2.shape
-    if x2.shape[0] != M:
-        raise RuntimeError(f"{name}: g has {M} rows, x {x2.shape[0]}")
-    K = x2.shape[1]
-    out = _new(K, N, torch.bfloat16, g.device) if transposed else _new(N, K, torch.bfloat16, g.device)
-    with _DeviceGuard(g):
-        ws, n = _workspace("ltxfp8_wgrad_workspace_bytes", (M, N, K), g.device)
-        L.check(L.load().ltxfp8_wgrad(g2.data_ptr(), _ld(g2), x2.data_ptr(), _ld(x2), _ptr(x_scales), x_ld,
-                                      float(alpha), out.data_ptr(), int(transposed), M, N, K, _ptr(ws), n, _stream(g)))
-    return out
+    return L.binding().act_backward(dy, z_q, z_scales, activation, quantize, dbias)
 
 
 def wgrad_1x128(g: torch.Tensor, x_q: torch.Tensor, x_scales: torch.Tensor, *, alpha: float = 1.0,
@@ -815,17 +611,12 @@ def wgrad_1x128(g: torch.Tensor, x_q: torch.Tensor, x_scales: torch.Tensor, *, a
     ``g`` bf16 [..., N] is the gradient of the layer's output (N a multiple of 16, so LoRA
     ranks fit), ``x_q``/``x_scales`` the input's e4m3 codes [..., K] and 1x128 scales, as the
     forward GEMM read them.  Codes are expanded to bf16 on their way into the tensor core."""
-    name = "wgrad_1x128"
-    _require_cuda(name, g, x_q, x_scales)
-    q2, x_scales, ld = _code_rows(x_q, x_scales, f"{name}: x")
-    return _wgrad(name, g, q2, x_scales, ld, alpha, transposed)
+    return L.binding().wgrad_1x128(g, x_q, x_scales, alpha, transposed)
 
 
 def wgrad_bf16(g: torch.Tensor, x: torch.Tensor, *, alpha: float = 1.0, transposed: bool = False) -> torch.Tensor:
     """:func:`wgrad_1x128` of a bf16 ``x`` [..., K], K a multiple of 128."""
-    name = "wgrad_bf16"
-    _require_cuda(name, g, x)
-    return _wgrad(name, g, _bf16_rows(x, f"{name}: x"), None, 0, alpha, transposed)
+    return L.binding().wgrad_bf16(g, x, alpha, transposed)
 
 
 def transpose_weight_128x128(w_q: torch.Tensor, sfb: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
