@@ -413,6 +413,15 @@ int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const
                  void* stream);
 int ltxfp8_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes);
 
+/* How ltxfp8_wgrad runs a shape on a GPU with `sms` multiprocessors; a host computation only. */
+typedef struct ltxfp8_wgrad_plan_info {
+  size_t workspace_bytes;
+  int pair;      /* 1: CTA pairs (512 x columns tiles), 0: single CTAs (256 x columns) */
+  int columns;   /* of g in a tile */
+  int splits;    /* of the M rows; above 1 a second launch adds the partial sums */
+} ltxfp8_wgrad_plan_info;
+int ltxfp8_wgrad_plan_for_sms(int64_t M, int64_t N, int64_t K, int sms, ltxfp8_wgrad_plan_info* info);
+
 /*
  * Transpose of a blockwise-FP8 weight for the input gradient dX = dY W: codes [N, K] ->
  * qt [K, N], scales [N/128, K/128] -> sfbt [K/128, N/128].  Not in place.

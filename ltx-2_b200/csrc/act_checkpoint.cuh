@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
     fence_mbarrier_init();
   }
   __syncthreads();
+  grid_launch_dependents();
   if (warp == 0)
     for (int j = 0; j < kActBwdStages && j < npass; ++j) load_pass(j);
 

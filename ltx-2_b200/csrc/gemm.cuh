@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (kAct >= 0) grid_launch_dependents();  // the split-K reduction, if there is one
 
   if (warp < 4) {
     setmaxnreg_dec<kRegsCtrl>();
@@ -679,6 +680,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmParams p) 
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  if constexpr (kAct >= 0) grid_wait_dependencies();
   if (active) {
     const int64_t split_stride = static_cast<int64_t>(kBM) * kBN;
     const float* src = p.ws + (static_cast<int64_t>(st) * p.k_splits * kBM + r) * kBN + g * 128 + l16 * 8;

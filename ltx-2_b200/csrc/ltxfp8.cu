@@ -70,9 +70,10 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2-D tensor map over a row-major [outer, inner] array, 128 B swizzle.
+// 2-D tensor map over a row-major [outer, inner] array, 128 B swizzle unless told otherwise.
 int make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
-                uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
+                uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
+                CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(LTXFP8_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
   cuuint64_t dims[2] = {inner, outer};
@@ -80,7 +81,7 @@ int make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(LTXFP8_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return LTXFP8_OK;
 }
@@ -93,7 +94,8 @@ struct DeviceInfo {
   bool pair_ready[4] = {false, false, false, false};
   int pair_clusters = 0;  // co-resident 2-CTA clusters of the pair kernel
   bool lora_ready = false;
-  bool wgrad_ready[2] = {false, false};  // by x type: bf16, e4m3
+  bool wgrad_ready[4] = {};              // by (x is e4m3, CTA pair)
+  int wgrad_clusters = 0;                // co-resident CTA pairs of the weight gradient
   bool norm_bwd_ready[6] = {};           // by (warps a row, runs a thread)
   bool act_bwd_ready[2] = {};            // by activation
   float* static_scratch = nullptr;  // device address of g_gemm_static_scratch (ltxfp8_gemm_static_scratch)
@@ -123,6 +125,24 @@ int device_info(DeviceInfo** out) {
                 d.minor);
   *out = &d;
   return LTXFP8_OK;
+}
+
+// Launch a kernel whose blocks may be scheduled while the previous kernel of the stream still
+// runs; it must call grid_wait_dependencies() before it touches that kernel's output.  The
+// start of the second kernel of a two-kernel operator then overlaps the first one's tail.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
 }
 
 template <bool kGelu, bool kRequant, int kAct = -1>
@@ -250,8 +270,13 @@ template <bool kGelu, bool kRequant, int kAct = -1>
 int splitk_reduce_launch(const DeviceInfo* d, const GemmParams& p, cudaStream_t stream) {
   const int64_t groups = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const unsigned blocks = static_cast<unsigned>((groups + 15) / 16);
-  splitk_reduce_kernel<kGelu, kRequant, kAct><<<blocks, 256, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if constexpr (kAct >= 0) {
+    e = launch_dependent(splitk_reduce_kernel<kGelu, kRequant, kAct>, blocks, 256, stream, p);
+  } else {
+    splitk_reduce_kernel<kGelu, kRequant, kAct><<<blocks, 256, 0, stream>>>(p);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return cuda_fail(e, "split-K reduce launch");
   (void)d;
   return LTXFP8_OK;
@@ -438,6 +463,46 @@ cudaError_t norm_bwd_launch(DeviceInfo* d, const NormBwdParams& p, unsigned grid
   if (e != cudaSuccess) return e;
   kern<<<grid, norm_threads<kWarps>, smem, s>>>(p);
   return cudaGetLastError();
+}
+
+template <bool kXFp8, bool kPair>
+cudaError_t wgrad_launch(DeviceInfo* d, const CUtensorMap& mx, const CUtensorMap& mg, const WgradParams& p,
+                         cudaStream_t s) {
+  auto kern = wgrad_kernel<kXFp8, kPair>;
+  cudaError_t e = allow_smem(kern, &d->wgrad_ready[(kXFp8 ? 2 : 0) | (kPair ? 1 : 0)], kWgSmemBytes);
+  if (e != cudaSuccess) return e;
+  const int units = p.k_tiles * p.n_tiles * p.splits;
+  if constexpr (!kPair) {
+    kern<<<units < d->sms ? units : d->sms, kWgThreads, kWgSmemBytes, s>>>(mx, mg, p);
+    return cudaGetLastError();
+  } else {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kWgThreads);
+    cfg.dynamicSmemBytes = kWgSmemBytes;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters;
+    {
+      // A persistent grid: as many pairs as can be resident.
+      std::lock_guard<std::mutex> lk(g_dev_mu);
+      if (d->wgrad_clusters == 0) {
+        cfg.gridDim = dim3(2 * (d->sms / 2));
+        e = cudaOccupancyMaxActiveClusters(&d->wgrad_clusters, kern, &cfg);
+        if (e != cudaSuccess) return e;
+        if (d->wgrad_clusters < 1) return cudaErrorInvalidConfiguration;
+      }
+      clusters = d->wgrad_clusters;
+    }
+    cfg.gridDim = dim3(2 * (units < clusters ? units : clusters));
+    return cudaLaunchKernelEx(&cfg, kern, mx, mg, p);
+  }
 }
 
 template <int kWarps, int kChunks>
@@ -1408,10 +1473,8 @@ int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64
   }
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward launch");
   if (dweight) {
-    col_sum_kernel<<<static_cast<unsigned>((H + 31) / 32), kColSumWarps * 32, 0, s>>>(p.dw_part, static_cast<int>(blocks),
-                                                                        static_cast<int>(H), dweight,
-                                                                        weight_dtype == LTXFP8_DTYPE_F32);
-    e = cudaGetLastError();
+    e = launch_dependent(col_sum_kernel, static_cast<unsigned>((H + 31) / 32), kColSumWarps * 32, s, p.dw_part,
+                         static_cast<int>(blocks), static_cast<int>(H), dweight, weight_dtype == LTXFP8_DTYPE_F32);
     if (e != cudaSuccess) return cuda_fail(e, "rms_norm_backward sum launch");
   }
   return LTXFP8_OK;
@@ -1557,9 +1620,8 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "act_backward launch");
   if (dbias) {
-    col_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), kColSumWarps * 32, 0, s>>>(p.db_part, pl.shares,
-                                                                        static_cast<int>(N), dbias, true);
-    e = cudaGetLastError();
+    e = launch_dependent(col_sum_kernel, static_cast<unsigned>((N + 31) / 32), kColSumWarps * 32, s, p.db_part,
+                         pl.shares, static_cast<int>(N), dbias, true);
     if (e != cudaSuccess) return cuda_fail(e, "act_backward sum launch");
   }
   return LTXFP8_OK;
@@ -1586,43 +1648,61 @@ int ltxfp8_transpose_weight_128x128(const void* q, const float* sfb, int64_t N, 
 }
 
 // ----------------------------------------------------------------------------- weight gradient
-// Tile width and splits of the summed axis.  A cost model in clock cycles picks among tile
-// widths (multiples of 16, at most 256; a single tile when N fits one) and splits: a stage
-// of 64 tokens costs the larger of its MMAs (4 cycles a column) and the expansion of its
-// codes, a unit has a fixed start and drain, and the units run in waves over the SMs; split
+// Kernel form, tile width and splits of the summed axis.  A cost model in clock cycles picks
+// among the one-CTA and the CTA-pair form, tile widths (multiples of 16, 64 to 256) and splits: a stage of 64 tokens costs what its form measured, a unit has a
+// fixed start and drain, the units run in waves over the SMs (or pairs of SMs), and split
 // partials are written and read back at L2 rates and cost one more launch.
+// Cycles of a 64-token stage, fitted to one CTA at nt = 128 / 240 (1112 / 1340) and a pair at
+// nt = 128 / 192 / 256 (1040 / 1120 / 1300).
+static double wgrad_stage_cycles(bool pair, int nt) { return pair ? 760.0 + 2.1 * nt : 860.0 + 2.0 * nt; }
+
 struct WgradPlan {
+  bool pair;
   int nt, n_tiles, k_tiles, stages, splits, per_split;
   size_t ws_bytes;
 };
 
 static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
-  // The plan of the last shape on this thread: a call asks for it twice (workspace, launch).
+  // Plans of this thread's recent shapes: a call asks twice (workspace, launch), and a training
+  // step repeats the same few shapes.
   static thread_local struct {
     int sms;
     int64_t M, N, K;
     WgradPlan plan;
-  } last{};
+  } recent[16] = {};
+  auto& last = recent[static_cast<uint64_t>(M * 31 + N * 7 + K) / 16 % 16];
   if (last.sms == sms && last.M == M && last.N == N && last.K == K) return last.plan;
   WgradPlan best{};
   double best_cost = 0.0;
-  const int64_t stages = (M + kWgStageM - 1) / kWgStageM, k_tiles = (K + kWgTileK - 1) / kWgTileK;
-  const int nt_hi = static_cast<int>(N < 256 ? N : 256), nt_lo = N <= 256 ? nt_hi : 128;
-  for (int nt = nt_hi; nt >= nt_lo; nt -= 16) {
-    const int64_t n_tiles = (N + nt - 1) / nt, tiles = n_tiles * k_tiles;
-    const int64_t max_s = stages < 64 ? stages : 64;
-    for (int64_t s = 1; s <= max_s; ++s) {
-      const int64_t per = (stages + s - 1) / s, used = (stages + per - 1) / per;
-      if (used != s) continue;
-      const double stage = 4.0 * nt > 700.0 ? 4.0 * nt : 700.0;
-      const double unit = static_cast<double>(per) * stage + 3000.0 + 16.0 * nt;
-      const int64_t waves = (tiles * s + sms - 1) / sms;
-      const double ws = s > 1 ? static_cast<double>(tiles * s) * nt * kWgTileK * 4.0 : 0.0;
-      const double cost = static_cast<double>(waves) * unit + (s > 1 ? 5000.0 + ws / 1500.0 : 0.0);
-      if (ws <= 512.0 * 1048576.0 && tiles * s <= 0x7FFFFFFF && (best.nt == 0 || cost < best_cost)) {
-        best_cost = cost;
-        best = WgradPlan{nt, static_cast<int>(n_tiles), static_cast<int>(k_tiles), static_cast<int>(stages),
-                         static_cast<int>(s), static_cast<int>(per), static_cast<size_t>(ws)};
+  const int64_t stages = (M + kWgStageM - 1) / kWgStageM;
+  const int nt_hi = static_cast<int>(N < 256 ? N : 256), nt_lo = N < 64 ? nt_hi : 64;
+  for (int pair = 0; pair < 2; ++pair) {
+    const int64_t k_tiles = (K + kWgTileK * (1 + pair) - 1) / (kWgTileK * (1 + pair));
+    const int64_t slots = sms / (1 + pair);
+    if (slots < 1) continue;
+    for (int nt = nt_hi; nt >= nt_lo; nt -= 16) {
+      if (pair && nt % 32 != 0) continue;  // each CTA of a pair holds nt / 2 columns, a multiple of 16
+      const int64_t n_tiles = (N + nt - 1) / nt, tiles = n_tiles * k_tiles;
+      const int64_t max_s = stages < 64 ? stages : 64;
+      for (int64_t s = 1; s <= max_s; ++s) {
+        const int64_t per = (stages + s - 1) / s, used = (stages + per - 1) / per;
+        if (used != s) continue;
+        const double stage = wgrad_stage_cycles(pair != 0, nt);
+        const double unit = static_cast<double>(per) * stage + 3000.0 + 16.0 * nt;
+        const int64_t waves = (tiles * s + slots - 1) / slots;
+        const double ws = s > 1 ? static_cast<double>(tiles * s) * (1 + pair) * nt * kWgTileK * 4.0 : 0.0;
+        const double cost = static_cast<double>(waves) * unit + (s > 1 ? 4000.0 + ws / 1500.0 : 0.0);
+        if (ws <= 512.0 * 1048576.0 && tiles * s <= 0x3FFFFFFF && (best.nt == 0 || cost < best_cost)) {
+          best_cost = cost;
+          best = WgradPlan{pair != 0,
+                           nt,
+                           static_cast<int>(n_tiles),
+                           static_cast<int>(k_tiles),
+                           static_cast<int>(stages),
+                           static_cast<int>(s),
+                           static_cast<int>(per),
+                           static_cast<size_t>(ws)};
+        }
       }
     }
   }
@@ -1632,6 +1712,29 @@ static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
   last.K = K;
   last.plan = best;
   return best;
+}
+
+// Stages of the kernel's rings in its 224 KB.  Codes: three operand stages (32 KB each; four
+// beside a g tile of one atom) cover the latency of expansion, MMAs and release, then four stages
+// of raw codes, or two where g would keep fewer than three.  Measured at 6144 x 4096 x 4096 in
+// cycles per 64 tokens, one CTA at nt = 240: operand/raw/g 3/2/3 1340, 2/4/3 1670, 3/4/2 1730;
+// a pair at nt = 256: 3/4/4 1300, 2/4/6 1490, 4/2/4 1340.  bf16 x: TMA fills the operand stages.
+static void wgrad_rings(WgradParams& p, bool fp8, bool pair) {
+  const uint32_t g_bytes = static_cast<uint32_t>((p.nt / (pair ? 2 : 1) + 63) / 64) * kWgAtomBytes;
+  if (!fp8) {
+    const int n = static_cast<int>(kWgRingBytes / (kWgOpBytes + g_bytes));
+    p.op_stages = p.g_stages = n < kWgMaxStages ? n : kWgMaxStages;
+    p.raw_stages = 0;
+    return;
+  }
+  p.op_stages = g_bytes <= kWgAtomBytes ? 4 : 3;
+  const uint32_t left = kWgRingBytes - static_cast<uint32_t>(p.op_stages) * kWgOpBytes;
+  for (const int raw : kWgRawStages) {
+    p.raw_stages = raw;
+    p.g_stages = static_cast<int>((left - static_cast<uint32_t>(raw) * kWgRawBytes) / g_bytes);
+    if (p.g_stages >= 3) break;
+  }
+  if (p.g_stages > kWgMaxStages) p.g_stages = kWgMaxStages;
 }
 
 static int wgrad_check(int64_t M, int64_t N, int64_t K) {
@@ -1651,6 +1754,20 @@ int ltxfp8_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes)
   rc = device_info(&d);
   if (rc) return rc;
   *bytes = wgrad_plan(d->sms, M, N, K).ws_bytes;
+  return LTXFP8_OK;
+}
+
+int ltxfp8_wgrad_plan_for_sms(int64_t M, int64_t N, int64_t K, int sms, ltxfp8_wgrad_plan_info* info) {
+  if (!info) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad_plan: null pointer");
+  memset(info, 0, sizeof(*info));
+  int rc = wgrad_check(M, N, K);
+  if (rc) return rc;
+  if (M < 1 || sms < 1) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "wgrad_plan: need M >= 1 and sms >= 1");
+  const WgradPlan pl = wgrad_plan(sms, M, N, K);
+  info->workspace_bytes = pl.ws_bytes;
+  info->pair = pl.pair ? 1 : 0;
+  info->columns = pl.nt;
+  info->splits = pl.splits;
   return LTXFP8_OK;
 }
 
@@ -1682,7 +1799,7 @@ int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const
   }
   const bool fp8 = xs != nullptr;
   CUtensorMap mx, mg;
-  if (fp8) rc = make_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, K, M, x_ld, 128, kWgStageM);
+  if (fp8) rc = make_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, K, M, x_ld, kWgTileK, kWgStageM, CU_TENSOR_MAP_SWIZZLE_NONE);
   else rc = make_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, K, M, x_ld * 2, 64, kWgStageM);
   if (rc) return rc;
   rc = make_map_2d(&mg, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g, N, M, g_ld * 2, 64, kWgStageM);
@@ -1705,25 +1822,15 @@ int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const
   p.ld_n = transposed ? 1 : K;
   p.ld_k = transposed ? N : 1;
   p.ws = static_cast<float*>(workspace);
-  {
-    std::lock_guard<std::mutex> lk(g_dev_mu);
-    if (!d->wgrad_ready[fp8]) {
-      cudaError_t e = fp8 ? cudaFuncSetAttribute(wgrad_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmemBytes)
-                          : cudaFuncSetAttribute(wgrad_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmemBytes);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(wgrad smem)");
-      d->wgrad_ready[fp8] = true;
-    }
-  }
-  const int units = pl.k_tiles * pl.n_tiles * pl.splits;
-  const int grid = units < d->sms ? units : d->sms;
-  if (fp8) wgrad_kernel<true><<<grid, kWgThreads, kWgSmemBytes, s>>>(mx, mg, p);
-  else wgrad_kernel<false><<<grid, kWgThreads, kWgSmemBytes, s>>>(mx, mg, p);
-  cudaError_t e = cudaGetLastError();
+  wgrad_rings(p, fp8, pl.pair);
+  cudaError_t e;
+  if (fp8) e = pl.pair ? wgrad_launch<true, true>(d, mx, mg, p, s) : wgrad_launch<true, false>(d, mx, mg, p, s);
+  else e = pl.pair ? wgrad_launch<false, true>(d, mx, mg, p, s) : wgrad_launch<false, false>(d, mx, mg, p, s);
   if (e != cudaSuccess) return cuda_fail(e, "wgrad launch");
   if (pl.splits > 1) {
-    const int64_t threads = static_cast<int64_t>(pl.k_tiles) * pl.n_tiles * pl.nt * (kWgTileK / 4);
-    wgrad_reduce_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p);
-    e = cudaGetLastError();
+    const int ctas = pl.pair ? 2 : 1;
+    const int64_t threads = static_cast<int64_t>(pl.k_tiles) * ctas * pl.n_tiles * pl.nt * (kWgTileK / 4);
+    e = launch_dependent(wgrad_reduce_kernel, static_cast<unsigned>((threads + 255) / 256), 256, s, p, ctas);
     if (e != cudaSuccess) return cuda_fail(e, "wgrad reduce launch");
   }
   return LTXFP8_OK;

@@ -37,6 +37,18 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
 
 __device__ __forceinline__ uint32_t lane_id() { return threadIdx.x & 31u; }
 
+// One lane of a converged warp.  Loops that the whole warp runs, with only the issue of a TMA
+// copy or an MMA under this predicate, keep their addresses and descriptors warp-uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r != 0;
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -282,6 +294,35 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same, publishing this thread's earlier writes to the threads of the cluster that wait
+// on the barrier with mbar_wait_cluster.
+__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// mbar_wait with acquire semantics over the cluster (arrivals come from the peer CTA too).
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, unsigned int code,
+                                                  unsigned long long limit_ns = kWaitLimitNs) {
+  unsigned long long t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    const unsigned long long t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > limit_ns) {
+      record_status(code);
+      return false;
+    }
+  }
+}
+
 // 2-D tile load into this CTA's shared memory whose completion is counted on the
 // mbarrier of the pair's leader CTA (no multicast: the tile lands only here).
 __device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t leader_mbar, void* smem_dst, int32_t c0,
@@ -336,6 +377,13 @@ __device__ __forceinline__ void tc_commit_pair_mc(uint64_t* bar, uint16_t cta_ma
                "h"(cta_mask)
                : "memory");
 }
+
+// ---------------------------------------------------------------- dependent launches
+// Lets a grid launched with launch_dependent() behind this one start (its blocks are
+// scheduled once every block of this grid has called this or exited).
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Waits until the grids this one depends on have completed and their writes are visible.
+__device__ __forceinline__ void grid_wait_dependencies() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- register control
 template <uint32_t N>

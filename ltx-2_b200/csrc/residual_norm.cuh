@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
     fence_mbarrier_init();
   }
   __syncthreads();
+  grid_launch_dependents();  // the grid is one wave: the column sums' blocks can only queue behind it
   if (warp == 0)
     for (int j = 0; j < p.stages && j < passes; ++j) load_pass(j);
 
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(kColSumWarps * 32) col_sum_kernel(const float*
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = blockIdx.x * 32 + lane;
   float s = 0.0f;
+  grid_wait_dependencies();
   if (n < N) {
 #pragma unroll 8
     for (int i = warp; i < parts; i += kColSumWarps) s += part[static_cast<int64_t>(i) * N + n];

@@ -10,13 +10,25 @@
 // bf16 copy of x exists in memory.
 //
 // Both operands have the summed axis as their row axis, so they are MN-major operands of
-// tcgen05.mma.kind::f16.  A CTA computes a 256 (k) x nt (n <= 256) tile as two M = 128
-// accumulators that share the g tile; 64 tokens a stage.
-//   warp 0      TMA producer: codes [64, 256] (16 KB) into the raw ring, g [64, nt] into its
-//               own ring (bf16 x: straight into the operand ring)
-//   warp 1      MMA issuer: 2 x 4 MMAs (M128 N=nt K16) a stage
-//   warps 4-19  two groups of 8 that expand alternate stages of raw codes into the swizzled
-//               MN-major operand tile; after the unit's last stage, all drain the accumulators
+// tcgen05.mma.kind::f16, 64 tokens a stage.  A CTA computes a 256 (k) x nt (n <= 256) tile as
+// two M = 128 accumulators that share the g tile.
+//   warp 0      TMA producer of x: codes [64, 256] (16 KB) into the raw ring (bf16 x: straight
+//               into the operand ring)
+//   warp 2      TMA producer of g [64, nt] into its own ring: a stage of codes is free as soon as
+//               its values are in registers, one of g only after its MMAs
+//   warp 1      MMA issuer: 2 x 4 MMAs (K16) a stage
+//   warps 4-19  two groups of 8 that expand alternate stages of codes into the swizzled MN-major
+//               operand ring; after the unit's last stage, all drain the accumulators
+// The producers' and the issuer's instructions share the schedulers with 16 busy warps (about
+// 100 cycles each at one thread a warp): their loops run warp-uniform, with as few copies and
+// waits as the layouts allow.
+// kPair: two CTAs of a cluster work on one 512 (k) x nt tile with cta_group::2 MMAs (M = 256):
+// each expands its own 256 k and loads half of the g tile, the leader issues the MMAs.  What
+// bounds the kernel for wide g is shared-memory bandwidth (128 B a cycle): per stage of 1024
+// MMA cycles at nt = 256 one CTA alone moves 48 KB of TMA writes, 48 KB of expansion and 96 KB
+// of operand reads (1500 cycles); in a pair the g tile is stored once per pair and each SM's
+// tensor core reads half of it: 144 KB (1150 cycles), and the traffic from L2 falls from 48 KB
+// to 32 KB a stage and SM.
 // The summed axis is divided among `splits` units where the tiles alone would not fill the
 // GPU; those write fp32 partials that wgrad_reduce_kernel adds in split order.
 #pragma once
@@ -25,20 +37,23 @@
 
 namespace ltxfp8 {
 
-constexpr int kWgTileK = 256;
+constexpr int kWgTileK = 256;  // of one CTA
 constexpr int kWgStageM = 64;
-constexpr int kWgGroups = 2;        // expanding warp groups; stage i belongs to group i % 2
-constexpr int kWgThreads = 128 + kWgGroups * 256;
-constexpr int kWgRawStages = 4;   // 16 KB each
-constexpr int kWgGStages = 3;     // 32 KB each
-constexpr int kWgOpStages = 2;    // 32 KB each (3 when x is bf16: no raw ring)
+constexpr int kWgExpandWarps = 16;
+constexpr int kWgGroups = 2;  // of expanding warps
+// A multiple of the groups, so that a raw slot always serves the same group: with an odd count a
+// group could run ahead, meet a slot whose earlier load (the other group's, completing late) is
+// still pending, and take the phase before that for its own.
+constexpr int kWgRawStages[2] = {4, 2};
+static_assert(kWgRawStages[0] % kWgGroups == 0 && kWgRawStages[1] % kWgGroups == 0, "a raw slot belongs to one group");
+constexpr int kWgGroupWarps = kWgExpandWarps / kWgGroups;
+constexpr int kWgThreads = 128 + kWgExpandWarps * 32;
+constexpr int kWgMaxStages = 8;   // of any ring
 constexpr uint32_t kWgRawBytes = kWgStageM * kWgTileK;
 constexpr uint32_t kWgOpBytes = kWgStageM * kWgTileK * 2;
-constexpr uint32_t kWgGBytes = kWgStageM * 256 * 2;
 constexpr uint32_t kWgAtomBytes = kWgStageM * 128;  // 64 M/N values x 64 tokens
-constexpr uint32_t kWgSmemBytes = kWgRawStages * kWgRawBytes + kWgOpStages * kWgOpBytes + kWgGStages * kWgGBytes +
-                                  1024 /*align*/ + 256 /*barriers*/;
-static_assert(kWgRawStages * kWgRawBytes >= kWgOpBytes, "the bf16 form's third operand stage takes the raw ring's place");
+constexpr uint32_t kWgRingBytes = 224 * 1024;       // all rings
+constexpr uint32_t kWgSmemBytes = kWgRingBytes + 1024 /*align*/ + 512 /*barriers*/;
 
 enum WgradStatus : unsigned int {
   kStWgProducer = 0x57010001u,
@@ -59,18 +74,32 @@ struct WgradParams {
   float alpha;
   __nv_bfloat16* out;  // element (n, k) at out[n * ld_n + k * ld_k]; one of the strides is 1
   int64_t ld_n, ld_k;
-  float* ws;  // splits > 1: partial of unit u at ws[u * nt * 256], row n, column k
+  float* ws;  // splits > 1: partial of unit u (and CTA r of a pair) at ws[(u * pair + r) * nt * 256], [n][k]
+  int op_stages, raw_stages, g_stages;  // of the rings (bf16 x: no raw ring)
+};
+
+// Position in a ring of n stages.
+struct RingPos {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++s == n) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
 };
 
 struct WgradUnit {
   int k0, n0, first, count;  // first token stage and their number
 };
 
-__device__ __forceinline__ WgradUnit wgrad_unit(int u, const WgradParams& p) {
+// `ctas`: CTAs that share a unit; k0 is the first one's.
+__device__ __forceinline__ WgradUnit wgrad_unit(int u, const WgradParams& p, int ctas) {
   const int tile = u / p.splits, split = u - tile * p.splits;
   const int nt = tile / p.k_tiles, kt = tile - nt * p.k_tiles;
   WgradUnit w;
-  w.k0 = kt * kWgTileK;
+  w.k0 = kt * kWgTileK * ctas;
   w.n0 = nt * p.nt;
   w.first = split * p.stages_per_split;
   w.count = min(p.stages_per_split, p.stages - w.first);
@@ -89,46 +118,53 @@ __device__ __forceinline__ void expand16(const uint4& v, float s, uint4& lo, uin
   hi = r.b;
 }
 
-template <bool kXFp8>
+// mbar_wait with one outcome for the warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+template <bool kXFp8, bool kPair>
 __global__ void __launch_bounds__(kWgThreads, 1)
     wgrad_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG,
                  const WgradParams p) {
-  constexpr int kOpStages = kXFp8 ? kWgOpStages : kWgOpStages + 1;
+  constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  uint8_t* s_op = smem;                                    // operand ring (x, bf16)
-  uint8_t* s_raw = s_op + kWgOpStages * kWgOpBytes;        // raw ring; the bf16 form's third operand stage
-  uint8_t* s_g = s_raw + kWgRawStages * kWgRawBytes;       // g ring
-  uint64_t* raw_full = reinterpret_cast<uint64_t*>(s_g + kWgGStages * kWgGBytes);
-  uint64_t* raw_empty = raw_full + kWgRawStages;
-  uint64_t* g_full = raw_empty + kWgRawStages;
-  uint64_t* g_empty = g_full + kWgGStages;
-  uint64_t* op_full = g_empty + kWgGStages;
-  uint64_t* op_empty = op_full + kWgOpStages + 1;
-  uint64_t* acc_full = op_empty + kWgOpStages + 1;
-  uint64_t* acc_empty = acc_full + 1;
+  const int g_cols = p.nt / kCtas;  // columns of g that this CTA loads
+  const int boxes = (g_cols + 63) / 64;
+  const uint32_t g_bytes = boxes * kWgAtomBytes;
+  uint8_t* s_op = smem;                                 // operand ring (x, bf16)
+  uint8_t* s_raw = s_op + p.op_stages * kWgOpBytes;     // raw ring (codes)
+  uint8_t* s_g = s_raw + p.raw_stages * kWgRawBytes;    // g ring
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + kWgRingBytes);
+  uint64_t* raw_empty = raw_full + kWgMaxStages;
+  uint64_t* g_full = raw_empty + kWgMaxStages;   // in a pair: the leader's are used
+  uint64_t* g_empty = g_full + kWgMaxStages;
+  uint64_t* op_full = g_empty + kWgMaxStages;    // in a pair: the leader's are used
+  uint64_t* op_empty = op_full + kWgMaxStages;
+  uint64_t* acc_full = op_empty + kWgMaxStages;
+  uint64_t* acc_empty = acc_full + 1;            // in a pair: the leader's is used
   uint64_t* drain = acc_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0);
   const int lane = static_cast<int>(lane_id());
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
+  const bool leader = rank == 0;
+  const int team = static_cast<int>(blockIdx.x) / kCtas, teams = static_cast<int>(gridDim.x) / kCtas;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kWgRawStages; ++s) {
+    for (int s = 0; s < kWgMaxStages; ++s) {
       mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], 8);
-    }
-    for (int s = 0; s < kWgGStages; ++s) {
+      mbar_init(&raw_empty[s], kWgGroupWarps);
       mbar_init(&g_full[s], 1);
       mbar_init(&g_empty[s], 1);
-    }
-    for (int s = 0; s < kOpStages; ++s) {
-      mbar_init(&op_full[s], kXFp8 ? 8 : 1);
+      mbar_init(&op_full[s], kXFp8 ? kWgGroupWarps * kCtas : 1);
       mbar_init(&op_empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, kWgGroups * 8);
+    mbar_init(acc_empty, kWgExpandWarps * kCtas);
     mbar_init(drain, 1);
     fence_mbarrier_init();
   }
@@ -137,177 +173,217 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     tma_prefetch_desc(&tmG);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
   }
+  __syncwarp();
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const int units = p.k_tiles * p.n_tiles * p.splits;
+  grid_launch_dependents();
 
-  if (warp == 0 && lane == 0) {
-    // -------------------------------------------------------------- TMA producer
-    const int boxes = (p.nt + 63) / 64;
-    uint32_t it = 0;
-    bool ok = true, x_sent = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const WgradUnit w = wgrad_unit(u, p);
-      const int halves = w.k0 + 128 < p.K ? 2 : 1;
-      for (int i = 0; i < w.count; ++i, ++it) {
+  if (warp == 0 || warp == 2) {
+    // -------------------------------------------------------------- TMA producers: x, g
+    // Columns beyond K or N and rows beyond M arrive as zeros.  In a pair the copies that the
+    // leader's MMAs wait for directly (g, bf16 x) complete on the leader's barriers.
+    const bool is_x = warp == 0;
+    const bool shared_bar = kPair && !(kXFp8 && is_x);
+    uint64_t* full = !is_x ? g_full : kXFp8 ? raw_full : op_full;
+    uint64_t* empty = !is_x ? g_empty : kXFp8 ? raw_empty : op_empty;
+    const int stages = !is_x ? p.g_stages : kXFp8 ? p.raw_stages : p.op_stages;
+    const uint32_t bytes = !is_x ? g_bytes : kXFp8 ? kWgRawBytes : kWgOpBytes;
+    uint8_t* ring = !is_x ? s_g : kXFp8 ? s_raw : s_op;
+    const uint32_t full_l = shared_bar ? mapa_shared(smem_u32(full), 0) : 0u;
+    RingPos pos;
+    uint32_t sent = 0;
+    bool ok = true;
+    for (int u = team; u < units && ok; u += teams) {
+      const WgradUnit w = wgrad_unit(u, p, kCtas);
+      const int col = is_x ? w.k0 + rank * kWgTileK : w.n0 + rank * g_cols;
+      const int copies = !is_x ? boxes : kXFp8 ? 1 : kWgTileK / 64;
+      for (int i = 0; i < w.count; ++i) {
         const int m0 = (w.first + i) * kWgStageM;
-        x_sent = false;
-        if constexpr (kXFp8) {
-          const uint32_t s = it % kWgRawStages, ph = (it / kWgRawStages) & 1u;
-          if (!mbar_wait(&raw_empty[s], ph ^ 1u, kStWgProducer)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&raw_full[s], halves * (kWgRawBytes / 2));
-          for (int h = 0; h < halves; ++h)
-            tma_load_2d(&tmX, &raw_full[s], s_raw + s * kWgRawBytes + h * (kWgRawBytes / 2), w.k0 + h * 128, m0);
-        } else {
-          const uint32_t s = it % kOpStages, ph = (it / kOpStages) & 1u;
-          if (!mbar_wait(&op_empty[s], ph ^ 1u, kStWgProducer)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&op_full[s], halves * (kWgOpBytes / 2));
-          for (int h = 0; h < 2 * halves; ++h)
-            tma_load_2d(&tmX, &op_full[s], s_op + s * kWgOpBytes + h * kWgAtomBytes, w.k0 + h * 64, m0);
-        }
-        x_sent = true;
-        const uint32_t s = it % kWgGStages, ph = (it / kWgGStages) & 1u;
-        if (!mbar_wait(&g_empty[s], ph ^ 1u, kStWgProducer)) {
+        if (!warp_wait(&empty[pos.s], pos.ph ^ 1u, kStWgProducer)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&g_full[s], boxes * kWgAtomBytes);
-        for (int b = 0; b < boxes; ++b)
-          tma_load_2d(&tmG, &g_full[s], s_g + s * kWgGBytes + b * kWgAtomBytes, w.n0 + b * 64, m0);
+        uint8_t* dst = ring + pos.s * bytes;
+        uint64_t* bar = &full[pos.s];
+        if (elect_one()) {
+          if (!shared_bar) mbar_arrive_expect_tx(bar, bytes);
+          else if (leader) mbar_arrive_expect_tx(bar, 2u * bytes);
+          const CUtensorMap* map = is_x ? &tmX : &tmG;
+          for (int b = 0; b < copies; ++b) {
+            if (kPair && shared_bar)
+              tma_load_2d_pair(map, full_l + pos.s * 8u, dst + b * kWgAtomBytes, col + b * 64, m0);
+            else
+              tma_load_2d(map, bar, dst + b * kWgAtomBytes, col + b * 64, m0);
+          }
+        }
+        __syncwarp();
+        pos.next(stages);
+        ++sent;
       }
     }
-    if (!ok) {
+    if (!ok && (!shared_bar || leader)) {
       // Let the loads already in flight land before the CTA exits.
-      const uint32_t x_it = it + (x_sent ? 1u : 0u);
-      const uint32_t xs = kXFp8 ? kWgRawStages : kOpStages;
-      uint64_t* xf = kXFp8 ? raw_full : op_full;
-      for (uint32_t i = x_it > xs ? x_it - xs : 0u; i < x_it; ++i) mbar_wait(&xf[i % xs], (i / xs) & 1u, kStWgDrain);
-      for (uint32_t i = it > kWgGStages ? it - kWgGStages : 0u; i < it; ++i)
-        mbar_wait(&g_full[i % kWgGStages], (i / kWgGStages) & 1u, kStWgDrain);
+      for (uint32_t i = sent > static_cast<uint32_t>(stages) ? sent - stages : 0u; i < sent; ++i)
+        warp_wait(&full[i % stages], (i / stages) & 1u, kStWgDrain);
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && leader) {
     // -------------------------------------------------------------- MMA issuer
     const uint32_t idesc =
-        make_idesc(1u, 128u, static_cast<uint32_t>(p.nt)) | kIdescAMnMajor | kIdescBMnMajor;
-    uint32_t it = 0, tcount = 0;
+        make_idesc(1u, 128u * kCtas, static_cast<uint32_t>(p.nt)) | kIdescAMnMajor | kIdescBMnMajor;
+    auto commit = [](uint64_t* bar) {
+      if constexpr (kPair) tc_commit_pair_mc(bar, 0x3);
+      else tc_commit(bar);
+    };
+    RingPos op, gp;
+    uint32_t tcount = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++tcount) {
-      const WgradUnit w = wgrad_unit(u, p);
+    for (int u = team; u < units && ok; u += teams, ++tcount) {
+      const WgradUnit w = wgrad_unit(u, p, kCtas);
       const int halves = w.k0 + 128 < p.K ? 2 : 1;
-      if (!mbar_wait(acc_empty, (tcount & 1u) ^ 1u, kStWgAccEmpty)) break;
+      if (!warp_wait(acc_empty, (tcount & 1u) ^ 1u, kStWgAccEmpty)) break;
       tc_fence_after_sync();
-      for (int i = 0; i < w.count; ++i, ++it) {
-        const uint32_t so = it % kOpStages, po = (it / kOpStages) & 1u;
-        const uint32_t sg = it % kWgGStages, pg = (it / kWgGStages) & 1u;
-        if (!mbar_wait(&g_full[sg], pg, kStWgMma) || !mbar_wait(&op_full[so], po, kStWgMma)) {
+      for (int i = 0; i < w.count; ++i) {
+        if (!warp_wait(&g_full[gp.s], gp.ph, kStWgMma) || !warp_wait(&op_full[op.s], op.ph, kStWgMma)) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint64_t bdesc = sw128_mnmajor_desc(smem_u32(s_g + sg * kWgGBytes), kWgAtomBytes);
-        for (int h = 0; h < halves; ++h) {
-          const uint64_t adesc =
-              sw128_mnmajor_desc(smem_u32(s_op + so * kWgOpBytes + h * (kWgOpBytes / 2)), kWgAtomBytes);
+        const uint64_t adesc = sw128_mnmajor_desc(smem_u32(s_op + op.s * kWgOpBytes), kWgAtomBytes);
+        const uint64_t bdesc = sw128_mnmajor_desc(smem_u32(s_g + gp.s * g_bytes), kWgAtomBytes);
+        if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)  // 16 tokens = 2048 B of every atom
-            mma_f16(tmem_base + h * 256, adesc + 128u * j, bdesc + 128u * j, idesc, (i > 0 || j > 0) ? 1u : 0u);
+          for (int h = 0; h < 2; ++h) {
+            if (h < halves) {
+#pragma unroll
+              for (int j = 0; j < kWgStageM / 16; ++j) {  // 16 tokens = 2048 B of every atom
+                const uint64_t ad = adesc + (kWgOpBytes / 2 / 16) * h + 128u * j, bd = bdesc + 128u * j;
+                const uint32_t acc = (i > 0 || j > 0) ? 1u : 0u;
+                if constexpr (kPair) mma_f16_pair(tmem_base + h * 256, ad, bd, idesc, acc);
+                else mma_f16(tmem_base + h * 256, ad, bd, idesc, acc);
+              }
+            }
+          }
+          commit(&op_empty[op.s]);
+          commit(&g_empty[gp.s]);
+          if (i == w.count - 1) commit(acc_full);
         }
-        tc_commit(&op_empty[so]);
-        tc_commit(&g_empty[sg]);
+        __syncwarp();
+        op.next(p.op_stages);
+        gp.next(p.g_stages);
       }
-      if (ok) tc_commit(acc_full);
     }
-    // Every MMA this thread issued has completed once `drain` flips.
-    tc_commit(drain);
-    mbar_wait(drain, 0u, kStWgDrain);
+    // Every MMA issued above has completed once `drain` flips (in both CTAs of a pair).
+    if (elect_one()) commit(drain);
+    __syncwarp();
+    warp_wait(drain, 0u, kStWgDrain);
   } else if (warp >= 4) {
     // -------------------------------------------------------------- expansion, epilogue
-    const int t = (static_cast<int>(threadIdx.x) - 128) & 255, grp = (warp - 4) >> 3;
-    const int c = t & 7, rsub = t >> 3;  // 16-code chunk of a 128-code row, row modulo 32
-    const int sp = warp & 3, half = ((warp - 4) >> 2) & 1;
-    uint32_t it = 0, tcount = 0;
+    const uint32_t op_full_l = kPair ? mapa_shared(smem_u32(op_full), 0) : 0u;
+    constexpr int kRowStep = kWgGroupWarps * 4;           // token rows a group covers at once
+    constexpr int kItems = 2 * kWgStageM / kRowStep;       // 16-code chunks of a thread and stage
+    const int grp = (warp - 4) / kWgGroupWarps;
+    const int t = (static_cast<int>(threadIdx.x) - 128) % (kWgGroupWarps * 32);
+    const int c = t & 7, row0 = t >> 3;  // chunk of each 128-code group, first token row of the stage
+    const int sp = warp & 3, half = ((warp - 4) >> 2) & 1, colhalf = (warp - 4) >> 3;
+    RingPos raw, op;
+    for (int j = 0; kXFp8 && j < grp; ++j) {  // group j starts j stages behind
+      raw.next(p.raw_stages);
+      op.next(p.op_stages);
+    }
+    uint32_t it = 0, tcount = 0;  // stages and units so far
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++tcount) {
-      const WgradUnit w = wgrad_unit(u, p);
+    for (int u = team; u < units && ok; u += teams, ++tcount) {
+      const WgradUnit w = wgrad_unit(u, p, kCtas);
+      const int k0 = w.k0 + rank * kWgTileK;
       if constexpr (kXFp8) {
-        // Item j of a thread: half j >> 1, token row (j & 1) * 32 + rsub.
-        const int g0 = w.k0 / 128;
-        auto load_scales = [&](int i, float(&s)[4]) {
+        const int g0 = k0 / 128;
+        // Item j of a thread: 128-code group j & 1, token row (j >> 1) * kRowStep + row0.
+        auto load_scales = [&](int i, float(&s)[kItems]) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int m = (w.first + i) * kWgStageM + (j & 1) * 32 + rsub, g = g0 + (j >> 1);
+          for (int j = 0; j < kItems; ++j) {
+            const int m = (w.first + i) * kWgStageM + (j >> 1) * kRowStep + row0, g = g0 + (j & 1);
             s[j] = (i < w.count && m < p.M && g < p.groups) ? __ldg(p.xs + static_cast<int64_t>(g) * p.xs_ld + m) : 0.0f;
           }
         };
-        float sc[4], nx[4];
-        int i = static_cast<int>(it + grp) & (kWgGroups - 1);  // this group's first stage of the unit
+        float sc[kItems], nx[kItems];
+        int i = static_cast<int>((grp + kWgGroups - it % kWgGroups) % kWgGroups);  // its first stage of the unit
         load_scales(i, sc);
-        const uint32_t it0 = it;
         for (; i < w.count; i += kWgGroups) {
-          it = it0 + i;
           load_scales(i + kWgGroups, nx);
-          const uint32_t sr = it % kWgRawStages, pr = (it / kWgRawStages) & 1u;
-          const uint32_t so = it % kOpStages, po = (it / kOpStages) & 1u;
-          if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[sr], pr, kStWgConvert)) ||
-              !__all_sync(0xffffffffu, mbar_wait(&op_empty[so], po ^ 1u, kStWgConvert))) {
+          if (!warp_wait(&raw_full[raw.s], raw.ph, kStWgConvert)) {
             ok = false;
             break;
           }
-          const uint8_t* src = s_raw + sr * kWgRawBytes;
-          uint8_t* dst = s_op + so * kWgOpBytes;
+          const uint8_t* src = s_raw + raw.s * kWgRawBytes + row0 * kWgTileK + c * 16;
+          uint8_t* dst = s_op + op.s * kWgOpBytes + (c >> 2) * kWgAtomBytes + row0 * 128;
+          uint4 v[kItems];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int h = j >> 1, row = (j & 1) * 32 + rsub;
-            if (g0 + h >= p.groups) break;  // block-uniform: the tile's second group is outside K
-            const uint4 v = *reinterpret_cast<const uint4*>(src + h * (kWgRawBytes / 2) + row * 128 + ((c ^ (row & 7)) * 16));
+          for (int j = 0; j < kItems; ++j)  // all loads before the first store, which they could alias
+            v[j] = *reinterpret_cast<const uint4*>(src + (j >> 1) * (kRowStep * kWgTileK) + (j & 1) * 128);
+          if (!warp_wait(&op_empty[op.s], op.ph ^ 1u, kStWgConvert)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive(&raw_empty[raw.s]);  // the warp's codes are in registers (the vote above)
+#pragma unroll
+          for (int j = 0; j < kItems; ++j) {
+            // (A group outside K expands to zeros: its codes arrived as zeros, its scale is 0.)
             uint4 lo, hi;
-            expand16(v, sc[j], lo, hi);
+            expand16(v[j], sc[j], lo, hi);
             // Chunk c covers k = 16 c .. 16 c + 15 of the group: atom c >> 2, 16-byte positions
             // 2 (c & 3) and + 1, swizzled by the row.  Lanes of the second atom write their odd
             // position first, so the eight lanes of a row touch all 32 banks at once.
-            uint8_t* atom = dst + h * (kWgOpBytes / 2) + (c >> 2) * kWgAtomBytes + row * 128;
-            const int q0 = 2 * (c & 3) + (c >> 2), q1 = 2 * (c & 3) + 1 - (c >> 2);
-            *reinterpret_cast<uint4*>(atom + ((q0 ^ (row & 7)) * 16)) = (c >> 2) ? hi : lo;
-            *reinterpret_cast<uint4*>(atom + ((q1 ^ (row & 7)) * 16)) = (c >> 2) ? lo : hi;
+            uint8_t* atom = dst + (j & 1) * (kWgOpBytes / 2) + (j >> 1) * (kRowStep * 128);
+            const int q0 = 2 * (c & 3) + (c >> 2), q1 = 2 * (c & 3) + 1 - (c >> 2), sw = row0 & 7;  // kRowStep % 8 == 0
+            *reinterpret_cast<uint4*>(atom + ((q0 ^ sw) * 16)) = (c >> 2) ? hi : lo;
+            *reinterpret_cast<uint4*>(atom + ((q1 ^ sw) * 16)) = (c >> 2) ? lo : hi;
           }
           fence_proxy_async_smem();  // the tensor core reads these bytes through the async proxy
           __syncwarp();
+          // The operand bytes are read by this SM's tensor core, through the async proxy that the
+          // fence above orders them for; to the leader of a pair the arrival is only a signal.
           if (lane == 0) {
-            mbar_arrive(&raw_empty[sr]);
-            mbar_arrive(&op_full[so]);
+            if constexpr (kPair) mbar_arrive_cluster(op_full_l + op.s * 8u);
+            else mbar_arrive(&op_full[op.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[j] = nx[j];
+          for (int j = 0; j < kItems; ++j) sc[j] = nx[j];
+#pragma unroll
+          for (int j = 0; j < kWgGroups; ++j) {
+            raw.next(p.raw_stages);
+            op.next(p.op_stages);
+          }
         }
         if (!ok) break;
-        it = it0 + w.count;
+        it += static_cast<uint32_t>(w.count);
       }
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full, tcount & 1u, kStWgAccFull))) {
         ok = false;
         break;
       }
       tc_fence_after_sync();
-      const int k = w.k0 + half * 128 + sp * 32 + lane;
-      const bool k_ok = w.k0 + half * 128 < p.K;  // warp-uniform: K % 128 == 0
+      const int k = k0 + half * 128 + sp * 32 + lane;
+      const bool k_ok = k0 + half * 128 < p.K;  // warp-uniform: K % 128 == 0
       if (k_ok) {
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(sp * 32) << 16) + half * 256;
-        for (int c0 = grp * 32; c0 < p.nt; c0 += 32 * kWgGroups) {  // columns past nt are stale and not stored
+        for (int c0 = colhalf * 32; c0 < p.nt; c0 += 64) {  // columns past nt are stale and not stored
           uint32_t r[32];
           tmem_ld_32x32b_x32(taddr + c0, r);
           tmem_wait_ld();
           if (p.splits > 1) {
-            float* wsu = p.ws + (static_cast<int64_t>(u) * p.nt + c0) * kWgTileK + half * 128 + sp * 32 + lane;
+            float* wsu = p.ws + (static_cast<int64_t>(u * kCtas + rank) * p.nt + c0) * kWgTileK + half * 128 + sp * 32 + lane;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (c0 + j < p.nt) wsu[static_cast<int64_t>(j) * kWgTileK] = __uint_as_float(r[j]);
@@ -339,35 +415,47 @@ __global__ void __launch_bounds__(kWgThreads, 1)
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster_release(mapa_shared(smem_u32(acc_empty), 0));
+        else mbar_arrive(acc_empty);
+      }
     }
   }
+  if constexpr (kPair) {
+    if (!leader && warp == 1) warp_wait(drain, 0u, kStWgDrain);  // the pair's MMAs read this CTA too
+  }
 
+  __syncwarp();
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync();  // no CTA leaves while its peer may still reach its memory
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
 // out = bf16(alpha * sum over splits of the partials), in split order: one thread per four
-// neighbouring k of one n.
-__global__ void __launch_bounds__(256) wgrad_reduce_kernel(const WgradParams p) {
+// neighbouring k of one n of one CTA tile.
+__global__ void __launch_bounds__(256) wgrad_reduce_kernel(const WgradParams p, int ctas) {
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int kq = static_cast<int>(id & 63);
   const int64_t rowid = id >> 6;
-  const int tile = static_cast<int>(rowid / p.nt), nr = static_cast<int>(rowid - static_cast<int64_t>(tile) * p.nt);
+  const int part = static_cast<int>(rowid / p.nt), nr = static_cast<int>(rowid - static_cast<int64_t>(part) * p.nt);
+  const int tile = part / ctas, rank = part - tile * ctas;
   if (tile >= p.k_tiles * p.n_tiles) return;
   const int ntile = tile / p.k_tiles, kt = tile - ntile * p.k_tiles;
-  const int n = ntile * p.nt + nr, k = kt * kWgTileK + kq * 4;
+  const int n = ntile * p.nt + nr, k = (kt * ctas + rank) * kWgTileK + kq * 4;
   if (n >= p.N || k >= p.K) return;
-  const int64_t stride = static_cast<int64_t>(p.nt) * kWgTileK;
-  const float* src = p.ws + static_cast<int64_t>(tile) * p.splits * stride + static_cast<int64_t>(nr) * kWgTileK + kq * 4;
+  const int64_t block = static_cast<int64_t>(p.nt) * kWgTileK;
+  const float* src = p.ws + (static_cast<int64_t>(tile) * p.splits * ctas + rank) * block +
+                     static_cast<int64_t>(nr) * kWgTileK + kq * 4;
+  grid_wait_dependencies();
   float4 s = *reinterpret_cast<const float4*>(src);
 #pragma unroll 4
   for (int i = 1; i < p.splits; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(src + i * stride);
+    const float4 v = *reinterpret_cast<const float4*>(src + i * ctas * block);
     s.x += v.x;
     s.y += v.y;
     s.z += v.z;

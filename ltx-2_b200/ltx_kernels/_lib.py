@@ -76,6 +76,15 @@ class GemmPlanInfo(ctypes.Structure):
     ]
 
 
+class WgradPlanInfo(ctypes.Structure):
+    _fields_ = [
+        ("workspace_bytes", ctypes.c_size_t),
+        ("pair", ctypes.c_int),
+        ("columns", ctypes.c_int),
+        ("splits", ctypes.c_int),
+    ]
+
+
 # name -> (restype, argtypes); the exported symbols of include/ltxfp8.h
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 _sz = ctypes.c_size_t
@@ -121,6 +130,7 @@ SIGNATURES = {
     "ltxfp8_act_backward_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_sz)]),
     "ltxfp8_wgrad": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _f32, _vp, _i32, _i64, _i64, _i64, _vp, _sz, _vp]),
     "ltxfp8_wgrad_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "ltxfp8_wgrad_plan_for_sms": (_i32, [_i64, _i64, _i64, _i32, ctypes.POINTER(WgradPlanInfo)]),
     "ltxfp8_transpose_weight_128x128": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     "ltxfp8_device_status": (_i32, [ctypes.POINTER(ctypes.c_uint), _i32, _vp]),
     "ltxfp8_selftest_wait_timeout": (_i32, [ctypes.c_ulonglong, ctypes.POINTER(ctypes.c_uint), _vp]),
