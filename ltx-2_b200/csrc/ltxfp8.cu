@@ -16,6 +16,7 @@
 #include "act_checkpoint.cuh"
 #include "gemm.cuh"
 #include "gemm_pair.cuh"
+#include "gemm_small.cuh"
 #include "lora.cuh"
 #include "producers.cuh"
 #include "ptx.cuh"
@@ -462,6 +463,16 @@ cudaError_t norm_bwd_launch(DeviceInfo* d, const NormBwdParams& p, unsigned grid
   cudaError_t e = allow_smem(kern, &d->norm_bwd_ready[kIdx], kNormRingBytes / (kWarps > 8 ? 1 : 2));
   if (e != cudaSuccess) return e;
   kern<<<grid, norm_threads<kWarps>, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+// K blocks in flight per warp: four of 16 weight rows (64 registers), two beside the fragments of
+// 16 tokens.
+template <int kAct>
+cudaError_t gemm_small_launch(const GemmSmallParams& p, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(p.N / kSmallRows);
+  if (p.M <= 8) gemm_small_kernel<kAct, 1, 4><<<grid, kSmallWarps * 32, 0, s>>>(p);
+  else gemm_small_kernel<kAct, 2, 2><<<grid, kSmallWarps * 32, 0, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -1260,6 +1271,14 @@ int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_
 }
 
 // ----------------------------------------------------------------------------- residual epilogue
+// Where the weight-streaming kernel runs instead of the tensor-core one (and its split-K
+// reduction).  Measured, weight from memory, streaming / tensor-core: 8 tokens 4096 x 4096
+// 6.8 / 12.3 us, 16384 x 4096 18.7 / 24.4, 4096 x 16384 20.0 / 21.4; 16 tokens 4096 x 4096
+// 7.6 / 12.5, 16384 x 4096 24.6 / 23.7; 32 tokens 4096 x 4096 12.1 / 13.3, 16384 x 4096 42 / 24.
+static bool gemm_small_wins(int64_t M, int64_t N, int64_t K) {
+  return M <= 8 || (M <= 16 && N * K <= (static_cast<int64_t>(1) << 25));
+}
+
 int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const void* W, const float* sfb,
                          const float* bias, const void* residual, int64_t residual_ld, void* D, int64_t M, int64_t N,
                          int64_t K, int activation, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1288,6 +1307,27 @@ int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const 
   e.workspace_bytes = workspace_bytes;
   const ResidualEpilogue re{activation, static_cast<const __nv_bfloat16*>(residual), residual_ld};
   auto s = static_cast<cudaStream_t>(stream);
+  if (gemm_small_wins(M, N, K)) {
+    GemmSmallParams p;
+    p.a = static_cast<const uint8_t*>(A);
+    p.sfa = sfa;
+    p.sfa_ld = sfa_ld;
+    p.w = static_cast<const uint8_t*>(W);
+    p.sfb = sfb;
+    p.bias = bias;
+    p.res = re.res;
+    p.res_ld = residual_ld;
+    p.d = static_cast<__nv_bfloat16*>(D);
+    p.M = static_cast<int>(M);
+    p.N = static_cast<int>(N);
+    p.K = static_cast<int>(K);
+    p.kb = static_cast<int>(K / 128);
+    cudaError_t e = activation == LTXFP8_ACT_GELU_TANH ? gemm_small_launch<kActGeluTanh>(p, s)
+                    : activation == LTXFP8_ACT_SILU    ? gemm_small_launch<kActSilu>(p, s)
+                                                       : gemm_small_launch<kActNone>(p, s);
+    if (e != cudaSuccess) return cuda_fail(e, "gemm_residual launch");
+    return LTXFP8_OK;
+  }
   const GemmPlan g = gemm_plan(d->sms, M, N, K);
   const size_t need = splitk_bytes(g);
   if (need == 0 || !workspace || need > workspace_bytes)
