@@ -385,7 +385,8 @@ int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const 
 
 /*
  * Activation with an 8-bit checkpoint of its input: (yq, ys) = 1x128 quant of act(z),
- * (zq, zs) = 1x128 quant of z.  z bf16 [M, N], N % 128 == 0; LTXFP8_ACT_GELU_TANH or _SILU.
+ * (zq, zs) = 1x128 quant of z (zq NULL: no checkpoint, zs unused).  z bf16 [M, N],
+ * N % 128 == 0; LTXFP8_ACT_GELU_TANH or _SILU.
  */
 int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, int activation, void* yq, float* ys,
                              int64_t ys_ld, void* zq, float* zs, int64_t zs_ld, void* stream);

@@ -62,14 +62,18 @@ def build_binding(force: bool = False) -> str:
     root = os.path.dirname(torch.__file__)
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     tmp = os.path.join(LIB_DIR, "_ltxfp8_torch.tmp.so")
+    # The system's g++, not $CXX: a compiler that links its own libstdc++ statically puts a second
+    # C++ runtime beside torch's, and an exception that crosses them ends the process.
     subprocess.check_call([
-        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         "-I" + INCLUDE, "-isystem", os.path.join(root, "include"),
         "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
         "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
         src, "-o", tmp, "-L" + LIB_DIR, "-l:libltxfp8.so", "-L" + os.path.join(root, "lib"),
         "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    if b"libstdc++.so" not in subprocess.check_output(["readelf", "-d", tmp]):
+        raise RuntimeError("the tensor-level binding must share torch's C++ runtime (libstdc++.so), but g++ linked its own")
     os.replace(tmp, BINDING_PATH)
     return BINDING_PATH
 

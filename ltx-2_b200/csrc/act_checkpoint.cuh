@@ -34,7 +34,7 @@ struct ActSaveParams {
   uint8_t* yq;
   float* ys;
   int64_t ys_ld;
-  uint8_t* zq;
+  uint8_t* zq;  // null: no checkpoint
   float* zs;
   int64_t zs_ld;
 };
@@ -66,15 +66,17 @@ __global__ void __launch_bounds__(256, 6) act_quantize_save_kernel(const ActSave
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = act_apply<kAct>(z[j]);
     float zi, yi;
-    const uint4 zc = quant_run16(z, zi);
     const uint4 yc = quant_run16(y, yi);
+    const int64_t off = row[u] * p.N + kb[u] * 128 + l8 * kRunLen;
     if (row[u] < p.M) {
-      const int64_t off = row[u] * p.N + kb[u] * 128 + l8 * kRunLen;
       *reinterpret_cast<uint4*>(p.yq + off) = yc;
-      *reinterpret_cast<uint4*>(p.zq + off) = zc;
-      if (l8 == 0) {
-        p.ys[static_cast<int64_t>(kb[u]) * p.ys_ld + row[u]] = yi;
-        p.zs[static_cast<int64_t>(kb[u]) * p.zs_ld + row[u]] = zi;
+      if (l8 == 0) p.ys[static_cast<int64_t>(kb[u]) * p.ys_ld + row[u]] = yi;
+    }
+    if (p.zq != nullptr) {
+      const uint4 zc = quant_run16(z, zi);
+      if (row[u] < p.M) {
+        *reinterpret_cast<uint4*>(p.zq + off) = zc;
+        if (l8 == 0) p.zs[static_cast<int64_t>(kb[u]) * p.zs_ld + row[u]] = zi;
       }
     }
   }

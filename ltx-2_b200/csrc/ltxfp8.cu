@@ -124,6 +124,14 @@ int device_info(DeviceInfo** out) {
   if (d.major != 10 || d.minor != 0)
     return fail(LTXFP8_ERR_DEVICE, "this library is built for sm_100a (B200); device %d is sm_%d%d", dev, d.major,
                 d.minor);
+  // The tensor-map encoder is a driver call and needs a current context.  A thread that has
+  // made no runtime call yet (autograd's backward threads) has none: select the device once.
+  static thread_local int t_context_device = -1;
+  if (t_context_device != dev) {
+    e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+    t_context_device = dev;
+  }
   *out = &d;
   return LTXFP8_OK;
 }
@@ -1546,7 +1554,7 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
   if (M == 0) return LTXFP8_OK;
   if ((rc = norm_rows(name, "z", z, z_ld, N)) != 0) return rc;
   if ((rc = act_codes(name, "y", yq, ys, ys_ld, M)) != 0) return rc;
-  if ((rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
+  if (zq && (rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
   const int64_t groups = N / 128;
   const int64_t blocks = (M * groups + kActSaveGroups - 1) / kActSaveGroups;
   if (blocks > 0x7FFFFFFF) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: M * N is too large", name);

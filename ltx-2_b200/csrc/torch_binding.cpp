@@ -315,17 +315,22 @@ PyObject* gemm_residual(PyObject* const* a) {
   return wrap(out);
 }
 
-// (z, activation)
+// (z, activation, save)
 PyObject* act_quantize_save(PyObject* const* a) {
   const char* name = "act_quantize_save";
   const Tensor z = tensor_arg(name, "z", a[0]);
   const c10::Device dev = one_device(name, {&z});
   const int act = activation_arg(name, a[1], false);
+  const bool save = bool_arg(a[2]);
   const Rows zr = bf16_rows(name, "z", z);
   const int64_t M = zr.M, N = zr.K;
   const c10::cuda::OptionalCUDAGuard guard(dev);
-  const Tensor yq = new_tensor(dev, {M, N}, at::kFloat8_e4m3fn), ys = new_scales(dev, M, N / 128),
-               zq = new_tensor(dev, {M, N}, at::kFloat8_e4m3fn), zs = new_scales(dev, M, N / 128);
+  const Tensor yq = new_tensor(dev, {M, N}, at::kFloat8_e4m3fn), ys = new_scales(dev, M, N / 128);
+  Tensor zq, zs;
+  if (save) {
+    zq = new_tensor(dev, {M, N}, at::kFloat8_e4m3fn);
+    zs = new_scales(dev, M, N / 128);
+  }
   abi(ltxfp8_act_quantize_save(zr.ptr(), zr.ld, M, N, act, data(yq), static_cast<float*>(data(ys)), align4(M), data(zq),
                                static_cast<float*>(data(zs)), align4(M), stream_of(dev)));
   return wrap_all({&yq, &ys, &zq, &zs});
@@ -424,7 +429,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<fn, n>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     LTXFP8_ENTRY(rms_norm_quantize, 5), LTXFP8_ENTRY(rms_norm_backward, 5), LTXFP8_ENTRY(gemm_residual, 9),
-    LTXFP8_ENTRY(act_quantize_save, 2), LTXFP8_ENTRY(act_backward, 6),      LTXFP8_ENTRY(wgrad_1x128, 5),
+    LTXFP8_ENTRY(act_quantize_save, 3), LTXFP8_ENTRY(act_backward, 6),      LTXFP8_ENTRY(wgrad_1x128, 5),
     LTXFP8_ENTRY(wgrad_bf16, 4),        LTXFP8_ENTRY(set_check, 1),         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ltxfp8_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -103,7 +103,11 @@ class BlockwiseFP8FeedForward(nn.Module):
 
 
 class BlockwiseFP8LoRALinear(BlockwiseFP8Linear):
-    """BlockwiseFP8Linear plus a runtime LoRA ``alpha * B (A x)`` (bf16 A ``[r, in]``, B ``[out, r]``)."""
+    """BlockwiseFP8Linear plus a runtime LoRA ``alpha * B (A x)`` (bf16 A ``[r, in]``, B ``[out, r]``).
+
+    The factors are frozen by default.  Where gradients are enabled and the input, a factor or
+    the bias requires one, the forward is :func:`training.fp8_linear_train`: differentiable,
+    keeping the input in 8 bits (``layer.lora_A.requires_grad_()`` starts a LoRA fine-tune)."""
 
     def __init__(self, in_features: int, out_features: int, rank: int, alpha: float = 1.0, bias: bool = True,
                  device=None, dtype=None):
@@ -118,4 +122,9 @@ class BlockwiseFP8LoRALinear(BlockwiseFP8Linear):
     def forward(self, x):
         if isinstance(x, tuple):
             raise RuntimeError("BlockwiseFP8LoRALinear needs the bf16 input for the LoRA term")
+        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad
+                                        or (self.bias is not None and self.bias.requires_grad)):
+            from .training import fp8_linear_train
+            return fp8_linear_train(x, (self.weight, self.weight_scale), self.bias,
+                                    lora=(self.lora_A, self.lora_B, self.alpha))
         return fp8_linear(x, self.weight, self.weight_scale, self.bias, lora=(self.lora_A, self.lora_B, self.alpha))

@@ -583,13 +583,14 @@ def gemm_residual(a_q: torch.Tensor, sfa: torch.Tensor, w_q: torch.Tensor, sfb: 
     return L.binding().gemm_residual(a_q, sfa, w_q, sfb, bias, residual, activation, out, split_k)
 
 
-def act_quantize_save(z: torch.Tensor, activation: str = "gelu_tanh"):
+def act_quantize_save(z: torch.Tensor, activation: str = "gelu_tanh", *, save: bool = True):
     """An activation with the 8-bit checkpoint of its input, in one pass over ``z`` bf16 [..., N].
 
     Returns ``(y_codes, y_scales, z_codes, z_scales)``: the 1x128 quantisation of ``act(z)``
     (``"gelu_tanh"`` or ``"silu"``), the next GEMM's operand, and that of ``z``, which is all
-    that :func:`act_backward` needs.  Codes are [M, N], scales (M, N/128)."""
-    return L.binding().act_quantize_save(z, activation)
+    that :func:`act_backward` needs (None with ``save=False``).  Codes are [M, N], scales
+    (M, N/128)."""
+    return L.binding().act_quantize_save(z, activation, save)
 
 
 def act_backward(dy: torch.Tensor, z_q: torch.Tensor, z_scales: torch.Tensor, activation: str = "gelu_tanh", *,
