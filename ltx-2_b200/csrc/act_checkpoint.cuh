@@ -34,7 +34,7 @@ struct ActSaveParams {
   uint8_t* yq;
   float* ys;
   int64_t ys_ld;
-  uint8_t* zq;  // null: no checkpoint
+  uint8_t* zq;  // kSave: the checkpoint
   float* zs;
   int64_t zs_ld;
 };
@@ -42,7 +42,7 @@ struct ActSaveParams {
 constexpr int kActSaveUnroll = 2;
 constexpr int kActSaveGroups = 32 * kActSaveUnroll;  // 1x128 groups of a 256-thread block
 
-template <int kAct>
+template <int kAct, bool kSave>
 __global__ void __launch_bounds__(256, 6) act_quantize_save_kernel(const ActSaveParams p) {
   const int64_t g0 = static_cast<int64_t>(blockIdx.x) * kActSaveGroups;
   const int64_t row0 = g0 / p.groups;
@@ -65,18 +65,17 @@ __global__ void __launch_bounds__(256, 6) act_quantize_save_kernel(const ActSave
     run_to_f2(v[u], z);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = act_apply<kAct>(z[j]);
-    float zi, yi;
+    float zi = 0.0f, yi;
+    uint4 zc;
+    if constexpr (kSave) zc = quant_run16(z, zi);
     const uint4 yc = quant_run16(y, yi);
-    const int64_t off = row[u] * p.N + kb[u] * 128 + l8 * kRunLen;
     if (row[u] < p.M) {
+      const int64_t off = row[u] * p.N + kb[u] * 128 + l8 * kRunLen;
       *reinterpret_cast<uint4*>(p.yq + off) = yc;
-      if (l8 == 0) p.ys[static_cast<int64_t>(kb[u]) * p.ys_ld + row[u]] = yi;
-    }
-    if (p.zq != nullptr) {
-      const uint4 zc = quant_run16(z, zi);
-      if (row[u] < p.M) {
-        *reinterpret_cast<uint4*>(p.zq + off) = zc;
-        if (l8 == 0) p.zs[static_cast<int64_t>(kb[u]) * p.zs_ld + row[u]] = zi;
+      if constexpr (kSave) *reinterpret_cast<uint4*>(p.zq + off) = zc;
+      if (l8 == 0) {
+        p.ys[static_cast<int64_t>(kb[u]) * p.ys_ld + row[u]] = yi;
+        if constexpr (kSave) p.zs[static_cast<int64_t>(kb[u]) * p.zs_ld + row[u]] = zi;
       }
     }
   }

@@ -1576,8 +1576,10 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
   p.zs_ld = zs_ld;
   auto s = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(blocks);
-  if (activation == LTXFP8_ACT_GELU_TANH) act_quantize_save_kernel<kActGeluTanh><<<grid, 256, 0, s>>>(p);
-  else act_quantize_save_kernel<kActSilu><<<grid, 256, 0, s>>>(p);
+  auto kern = activation == LTXFP8_ACT_GELU_TANH
+                  ? (zq ? act_quantize_save_kernel<kActGeluTanh, true> : act_quantize_save_kernel<kActGeluTanh, false>)
+                  : (zq ? act_quantize_save_kernel<kActSilu, true> : act_quantize_save_kernel<kActSilu, false>);
+  kern<<<grid, 256, 0, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "act_quantize_save launch");
   return LTXFP8_OK;
