@@ -349,7 +349,7 @@ int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_
  * RMS norm with the residual's addition: h = bf16(x + residual) (h = x when residual is
  * NULL; then h must be NULL), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight;
  * with q != NULL (q, sfa) = 1x128 quant of y, otherwise out = bf16(y).  h may be x or
- * residual (in place).  weight [H] of weight_dtype (LTXFP8_DTYPE_F32 or _BF16) or NULL;
+ * residual when that is contiguous (in place).  weight [H] of weight_dtype (LTXFP8_DTYPE_F32 or _BF16) or NULL;
  * rstd fp32 [M] or NULL.  H % 128 == 0, H <= 16384.
  */
 int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int64_t M,
@@ -376,7 +376,8 @@ int ltxfp8_rms_norm_backward_workspace_bytes(int64_t M, int64_t H, size_t* bytes
 /*
  * ltxfp8_gemm with activation and residual in its epilogue, rounded once:
  *   D = bf16( act( sum_kb sfa[m,kb] sfb[n/128,kb] (A W^T)_kb + bias ) + residual )
- * residual bf16 [M, N] with row stride residual_ld (a multiple of 8), or NULL; it may be D.
+ * residual bf16 [M, N] with row stride residual_ld (a multiple of 8), or NULL; it may be D when contiguous.
+ * Up to 16 tokens a weight-streaming kernel runs (one launch, no workspace used).
  * workspace: split-K scratch of ltxfp8_gemm_workspace_bytes, optional as for ltxfp8_gemm.
  */
 int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const void* W, const float* sfb,

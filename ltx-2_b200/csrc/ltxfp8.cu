@@ -1300,6 +1300,8 @@ int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const 
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: unknown activation %d", activation);
   if (!A || !sfa || !W || !sfb || !D) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: null operand");
   if (sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: sfa_ld < M");
+  if (residual == D && residual_ld != N)
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: in place needs contiguous rows");
   if (residual && residual_ld < N) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: residual_ld < N");
   if (!aligned(A, 16) || !aligned(W, 16) || !aligned(D, 16) || (bias && !aligned(bias, 16)))
     return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: A, W, D and bias must be 16-byte aligned");
@@ -1384,6 +1386,8 @@ int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, 
   if (residual) {
     if ((rc = norm_rows(name, "residual", residual, residual_ld, H)) != 0) return rc;
     if ((rc = norm_rows(name, "h", h, H, H)) != 0) return rc;
+    if ((h == x && x_ld != H) || (h == residual && residual_ld != H))
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: in place needs contiguous rows", name);
   } else if (h) {
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: h is only written with a residual", name);
   }
@@ -1474,6 +1478,8 @@ int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64
   if (dh && (rc = norm_rows(name, "dh", dh, dh_ld, H)) != 0) return rc;
   if ((rc = norm_rows(name, "dx", dx, H, H)) != 0) return rc;
   if (!rstd) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: rstd is null", name);
+  if (dx == h || (dx == dy && dy_ld != H) || (dx == dh && dh_ld != H))
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: dx may only be dy or dh, with contiguous rows", name);
   if (!aligned(rstd, 4) || (dweight && !aligned(dweight, 4)))
     return fail(LTXFP8_ERR_MISALIGNED, "%s: rstd and dweight must be 4-byte aligned", name);
   DeviceInfo* d;
@@ -1633,6 +1639,7 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   if ((rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
   if (!dz && !dzq) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: need dz or dzq", name);
   if (dz && (rc = norm_rows(name, "dz", dz, N, N)) != 0) return rc;
+  if (dz == dy && dy_ld != N) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: in place needs contiguous rows", name);
   if (dzq && (rc = act_codes(name, "dz", dzq, dzs, dzs_ld, M)) != 0) return rc;
   DeviceInfo* d;
   rc = device_info(&d);

@@ -121,6 +121,20 @@ def test_wgrad_plan(M, N, K):
     assert lib.ltxfp8_wgrad_plan_for_sms(M, N, K, 0, ctypes.byref(i)) == L.ERR_INVALID_ARGUMENT
 
 
+def test_in_place_needs_contiguous_rows():
+    """Writing a result over a strided operand would overwrite its neighbours: refused."""
+    L, lib = _lib()
+    A = L.ERR_INVALID_ARGUMENT
+    Q = 2 * P
+    for h, xld, rld in ((P, 512, 256), (Q, 256, 512)):
+        assert lib.ltxfp8_rms_norm_quantize(P, xld, Q, rld, 4, 256, None, 0, 1e-6, h, 3 * P, P, 4, None, None, None) == A
+    for dx, h, dy_ld, dh_ld in ((P, Q, 512, 256), (3 * P, Q, 256, 512), (Q, Q, 256, 256)):
+        assert lib.ltxfp8_rms_norm_backward(P, dy_ld, h, 256, P, None, 0, 3 * P, dh_ld, 4, 256, dx, None, None, 0,
+                                            None) == A
+    assert lib.ltxfp8_gemm_residual(P, P, 8, P, P, None, Q, 512, Q, 8, 256, 256, 0, None, 0, None) == A
+    assert lib.ltxfp8_act_backward(P, 512, Q, P, 4, 4, 256, 1, P, None, None, 4, None, None, 0, None) == A
+
+
 def test_quantize_modes():
     L, lib = _lib()
     for mode, ok in ((L.QUANT_FINITE, True), (3, False)):
