@@ -75,7 +75,7 @@ def test_rms_norm_backward_refusals(kw, code):
 ])
 def test_gemm_residual_refusals(kw, code):
     L, lib = _lib()
-    a = dict(M=8, N=256, K=256, sfa_ld=8, r=P, r_ld=256, bias=None, D=P, act=0)
+    a = dict(M=8, N=256, K=256, sfa_ld=8, r=P, r_ld=256, bias=None, D=2 * P, act=0)
     a.update(kw)
     rc = lib.ltxfp8_gemm_residual(P, P, a["sfa_ld"], P, P, a["bias"], a["r"], a["r_ld"], a["D"], a["M"], a["N"], a["K"],
                                   a["act"], None, 0, None)
