@@ -257,6 +257,12 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
   if (warp == 0)
     for (int j = 0; j < p.stages && j < passes; ++j) load_pass(j);
 
+  // The gain stays in registers (16 a thread): its first load overlaps the first rows', and the
+  // passes need none.  With two runs a thread there is no room, and it is read per row.
+  constexpr bool kHoldGain = kChunks == 1;
+  float2 gain[kHoldGain ? 1 : kChunks][8];
+  if constexpr (kHoldGain) ld_gain(p.w, p.w_f32, t * kRunLen < p.H ? t * kRunLen : 0, gain[0]);
+
   float2 dw[kChunks][8];
 #pragma unroll
   for (int i = 0; i < kChunks; ++i)
@@ -285,15 +291,15 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
       vy[i] = in ? ld_run(v) : zero_run();
       vh[i] = in ? ld_run(v + p.H) : zero_run();
       vd[i] = (in && inputs == 3) ? ld_run(v + 2 * p.H) : zero_run();
-      float2 y[8], x[8], w[8], s = make_float2(0.0f, 0.0f);
+      float2 y[8], x[8], s = make_float2(0.0f, 0.0f);
       run_to_f2(vy[i], y);
       run_to_f2(vh[i], x);
-      ld_gain(p.w, p.w_f32, col < p.H ? col : 0, w);
+      if constexpr (!kHoldGain) ld_gain(p.w, p.w_f32, col < p.H ? col : 0, gain[i]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float2 yx = __fmul2_rn(y[k], __fmul2_rn(x[k], r2));  // dy * xhat
         dw[i][k] = __fadd2_rn(dw[i][k], yx);
-        s = __ffma2_rn(yx, w[k], s);
+        s = __ffma2_rn(yx, gain[kHoldGain ? 0 : i][k], s);
       }
       acc += s.x + s.y;
     }
@@ -310,14 +316,14 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int col = (i * kWarps * 32 + t) * kRunLen;
-      float2 y[8], x[8], w[8], d[8];
+      float2 y[8], x[8], d[8];
       run_to_f2(vy[i], y);
       run_to_f2(vh[i], x);
       run_to_f2(vd[i], d);
-      ld_gain(p.w, p.w_f32, col < p.H ? col : 0, w);
+      if constexpr (!kHoldGain) ld_gain(p.w, p.w_f32, col < p.H ? col : 0, gain[i]);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        d[k] = __ffma2_rn(r2, __ffma2_rn(__fmul2_rn(x[k], r2), c2, __fmul2_rn(y[k], w[k])), d[k]);
+        d[k] = __ffma2_rn(r2, __ffma2_rn(__fmul2_rn(x[k], r2), c2, __fmul2_rn(y[k], gain[kHoldGain ? 0 : i][k])), d[k]);
       if (row_ok && col < p.H) st_run(p.dx + row * p.H + col, f2_to_run(d));
     }
   }
