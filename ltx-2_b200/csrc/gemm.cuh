@@ -307,7 +307,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp < 4) {
     setmaxnreg_dec<kRegsCtrl>();
-    if (warp == 0 && lane == 0) {
+    // The producer's and the issuer's loops run warp-uniform, one elected lane issuing (2-3 %
+    // faster than one thread of each warp: 6144 x 4096 x 4096 103 -> 100 us).
+    if (warp == 0) {
       // ------------------------------------------------------------ TMA producer
       uint32_t it = 0;
       bool ok = true;
@@ -318,29 +320,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int m0 = w.mt * kBM, n0 = w.nt * kBN;
         for (int kb = 0; kb < w.n_blocks; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
-          if (!mbar_wait(&empty[s], ph ^ 1u, kStProducerEmpty)) {
+          if (!warp_wait(&empty[s], ph ^ 1u, kStProducerEmpty)) {
             ok = false;
             break;
           }
           uint8_t* sa = smem + s * kStageBytes;
           uint8_t* sb = sa + kABytes;
-          mbar_arrive_expect_tx(&full[s], kb < w.n_fp8 ? tx_fp8 : kStageBytes);
-          if (kb < w.n_fp8) {
-            tma_load_2d(&tmA, &full[s], sa, (w.kb_begin + kb) * kBK, m0);
-            tma_load_2d(&tmB, &full[s], sb, (w.kb_begin + kb) * kBK, n0);
-          } else {
-            const int c = (kb - w.n_fp8) * kLoraChunk;
-            tma_load_2d(&tmLX, &full[s], sa, c, m0);
-            tma_load_2d(&tmLB, &full[s], sb, c, n0);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[s], kb < w.n_fp8 ? tx_fp8 : kStageBytes);
+            if (kb < w.n_fp8) {
+              tma_load_2d(&tmA, &full[s], sa, (w.kb_begin + kb) * kBK, m0);
+              tma_load_2d(&tmB, &full[s], sb, (w.kb_begin + kb) * kBK, n0);
+            } else {
+              const int c = (kb - w.n_fp8) * kLoraChunk;
+              tma_load_2d(&tmLX, &full[s], sa, c, m0);
+              tma_load_2d(&tmLB, &full[s], sb, c, n0);
+            }
           }
+          __syncwarp();
         }
       }
       if (!ok) {
         // Let the loads already in flight land before the CTA exits.
         const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
-        for (uint32_t i = first; i < it; ++i) mbar_wait(&full[i % kStages], (i / kStages) & 1u, kStDrain);
+        for (uint32_t i = first; i < it; ++i) warp_wait(&full[i % kStages], (i / kStages) & 1u, kStDrain);
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
       constexpr uint32_t kIdescF8 = make_idesc(0u, kBM, kBN);
       constexpr uint32_t kIdescBF16 = make_idesc(1u, kBM, kBN);
@@ -353,12 +358,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int kb = 0; kb < w.n_blocks; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
           const uint32_t buf = it & 1u, bph = (it >> 1) & 1u;
-          if (!mbar_wait(&tempty[buf], bph ^ 1u, kStMmaTmemEmpty)) {
+          if (!warp_wait(&tempty[buf], bph ^ 1u, kStMmaTmemEmpty)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          if (!mbar_wait(&full[s], ph, kStMmaFull)) {
+          if (!warp_wait(&full[s], ph, kStMmaFull)) {
             ok = false;
             break;
           }
@@ -367,27 +372,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint64_t adesc = sw128_kmajor_desc(a_addr);
           const uint64_t bdesc = sw128_kmajor_desc(a_addr + kABytes);
           const uint32_t d_tmem = tmem_base + buf * kBN;
-          if (kb < w.n_fp8) {
+          if (elect_one()) {
+            if (kb < w.n_fp8) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)  // 4 x K32 (32 B of each 128 B row)
-              mma_f8f6f4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc_f8, j > 0 ? 1u : 0u);
-          } else {
+              for (int j = 0; j < 4; ++j)  // 4 x K32 (32 B of each 128 B row)
+                mma_f8f6f4(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc_f8, j > 0 ? 1u : 0u);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)  // 4 x K16 bf16 (32 B of each 128 B row)
-              mma_f16(d_tmem, adesc + 2u * j, bdesc + 2u * j, kIdescBF16, j > 0 ? 1u : 0u);
+              for (int j = 0; j < 4; ++j)  // 4 x K16 bf16 (32 B of each 128 B row)
+                mma_f16(d_tmem, adesc + 2u * j, bdesc + 2u * j, kIdescBF16, j > 0 ? 1u : 0u);
+            }
+            tc_commit(&empty[s]);
+            tc_commit(&tfull[buf]);
           }
-          tc_commit(&empty[s]);
-          tc_commit(&tfull[buf]);
+          __syncwarp();
         }
       }
-      // Every MMA this thread issued has completed once `drain` flips.
-      tc_commit(drain);
-      mbar_wait(drain, 0u, kStDrain);
+      // Every MMA issued above has completed once `drain` flips.
+      if (elect_one()) tc_commit(drain);
+      __syncwarp();
+      warp_wait(drain, 0u, kStDrain);
     } else if (warp >= 2 && p.k_splits == 1) {
       // ------------------------------------------------------------ staging -> global (warps 2, 3)
-      // (Whole warps 2 and 3 only: lanes 1-31 of warps 0 and 1 must not enter,
-      // their lane 0 never joins the warp-wide votes below.)  Warp pw owns the
-      // 32-row slices pw*32 and 64 + pw*32 of the tile: its passes and stores need
+      // Warp pw owns the 32-row slices pw*32 and 64 + pw*32 of the tile: its passes and stores need
       // no synchronisation with the other store warp.  Lane 0 issues the TMA stores.
       const int pw = warp - 2;
       const bool write_d = (p.flags & kGemmWriteD) != 0;

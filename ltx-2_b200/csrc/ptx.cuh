@@ -94,6 +94,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   }
 }
 
+// mbar_wait with one outcome for the warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

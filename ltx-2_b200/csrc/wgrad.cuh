@@ -118,11 +118,6 @@ __device__ __forceinline__ void expand16(const uint4& v, float s, uint4& lo, uin
   hi = r.b;
 }
 
-// mbar_wait with one outcome for the warp.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
-}
-
 template <bool kXFp8, bool kPair>
 __global__ void __launch_bounds__(kWgThreads, 1)
     wgrad_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG,
