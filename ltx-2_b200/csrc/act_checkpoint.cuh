@@ -111,7 +111,10 @@ constexpr uint32_t kActBwdDyBytes = kActBwdMaxGroups * 256;                    /
 constexpr uint32_t kActBwdStageBytes = kActBwdDyBytes + kActBwdMaxGroups * 128;  // + 4 KB of codes
 constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 72 KB: three blocks an SM
 
-template <int kAct>
+//
+// kDirect: a few rows (one share, so no partial sums and no second launch): the loads go straight
+// to registers.
+template <int kAct, bool kDirect>
 __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[kActBwdStages], freed[kActBwdStages];
@@ -126,7 +129,9 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
   const int npass = (p.passes - static_cast<int>(blockIdx.y) + static_cast<int>(gridDim.y) - 1) /
                     static_cast<int>(gridDim.y);
 
-  // Warp 0: fetch pass j of this block, two copies a row (its dy, its codes), one row a lane.
+  // Warp 0: fetch pass j of this block, its dy and its codes: one copy each where the block's rows
+  // are contiguous, else one per row and lane (many small copies cost more than their bytes).
+  const bool whole_q = p.col_groups == p.groups, whole_y = whole_q && p.dy_ld == p.N;
   auto load_pass = [&](int j) {
     const int s = j % kActBwdStages;
     const int64_t m0 = (blockIdx.y + static_cast<int64_t>(j) * gridDim.y) * p.rows;
@@ -136,8 +141,12 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
     if (lane < rows) {
       uint8_t* st = ring + s * kActBwdStageBytes;
       const int64_t m = m0 + lane;
-      bulk_load(&full[s], st + lane * p.col_groups * 256, p.dy + m * p.dy_ld + col0, ngroups * 256u);
-      bulk_load(&full[s], st + kActBwdDyBytes + lane * p.col_groups * 128, p.zq + m * p.N + col0, ngroups * 128u);
+      if (!whole_y || lane == 0)
+        bulk_load(&full[s], st + lane * p.col_groups * 256, p.dy + m * p.dy_ld + col0,
+                  ngroups * 256u * (whole_y ? rows : 1));
+      if (!whole_q || lane == 0)
+        bulk_load(&full[s], st + kActBwdDyBytes + lane * p.col_groups * 128, p.zq + m * p.N + col0,
+                  ngroups * 128u * (whole_q ? rows : 1));
     }
   };
   if (threadIdx.x == 0) {
@@ -148,9 +157,11 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
     fence_mbarrier_init();
   }
   __syncthreads();
-  grid_launch_dependents();
-  if (warp == 0)
-    for (int j = 0; j < kActBwdStages && j < npass; ++j) load_pass(j);
+  if constexpr (!kDirect) {
+    grid_launch_dependents();
+    if (warp == 0)
+      for (int j = 0; j < kActBwdStages && j < npass; ++j) load_pass(j);
+  }
 
   float2 db[8];
 #pragma unroll
@@ -166,16 +177,23 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
     const bool in = mine && m < p.M;
     const float sc = sc_next;
     sc_next = (mine && m + step < p.M) ? __ldg(zs + m + step) : 0.0f;
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, kStActLoad))) break;
-    const uint8_t* st = ring + s * kActBwdStageBytes;
     Run16 vy = zero_run();
     uint4 vz = make_uint4(0, 0, 0, 0);
-    if (in) {
-      vy = ld_run(reinterpret_cast<const __nv_bfloat16*>(st) + threadIdx.x * kRunLen);
-      vz = *reinterpret_cast<const uint4*>(st + kActBwdDyBytes + threadIdx.x * kRunLen);
+    if constexpr (kDirect) {
+      if (in) {
+        vy = ld_run(p.dy + m * p.dy_ld + col);
+        vz = *reinterpret_cast<const uint4*>(p.zq + m * p.N + col);
+      }
+    } else {
+      if (!warp_wait(&full[s], ph, kStActLoad)) break;
+      const uint8_t* st = ring + s * kActBwdStageBytes;
+      if (in) {
+        vy = ld_run(reinterpret_cast<const __nv_bfloat16*>(st) + threadIdx.x * kRunLen);
+        vz = *reinterpret_cast<const uint4*>(st + kActBwdDyBytes + threadIdx.x * kRunLen);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&freed[s]);
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&freed[s]);
     float2 d[8], z[8];
     run_to_f2(vy, d);
     codes16_to_f2(vz, z);
@@ -194,15 +212,15 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
         if ((t & 7) == 0) p.dzs[static_cast<int64_t>(kb) * p.dzs_ld + m] = inv;
       }
     }
-    if (warp == 0 && j + kActBwdStages < npass) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&freed[s], ph, kStActFree))) break;
+    if (!kDirect && warp == 0 && j + kActBwdStages < npass) {
+      if (!warp_wait(&freed[s], ph, kStActFree)) break;
       load_pass(j + kActBwdStages);
     }
   }
-  if (j < npass && warp == 0) {
+  if (!kDirect && j < npass && warp == 0) {
     // A wait gave up: let the copies already issued land before the block exits.
     const int issued = j + kActBwdStages < npass ? j + kActBwdStages : npass;
-    for (int i = j; i < issued; ++i) mbar_wait(&full[i % kActBwdStages], (i / kActBwdStages) & 1u, kStActDrain);
+    for (int i = j; i < issued; ++i) warp_wait(&full[i % kActBwdStages], (i / kActBwdStages) & 1u, kStActDrain);
   }
   __syncthreads();
   if (p.db_part == nullptr) return;

@@ -1593,20 +1593,31 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
 
 // Blocks of the activation's backward: column blocks of up to 4096 columns, evenly divided,
 // times row shares that make up what is resident at once (three blocks an SM).
+// Up to 64 rows the blocks are one group wide and take all rows, 32 at a time: one launch, and
+// the bias gradient needs no partial sums.
 struct ActBwdPlan {
+  bool direct;
   int col_groups, col_blocks, rows, passes, shares;
 };
+
+constexpr int64_t kActBwdDirectRows = 64;
 
 static ActBwdPlan act_bwd_plan(int sms, int64_t M, int64_t N) {
   ActBwdPlan a;
   const int64_t groups = N / 128;
-  a.col_blocks = static_cast<int>((groups + kActBwdMaxGroups - 1) / kActBwdMaxGroups);
+  a.direct = M <= kActBwdDirectRows;
+  a.col_blocks = static_cast<int>(a.direct ? groups : (groups + kActBwdMaxGroups - 1) / kActBwdMaxGroups);
   a.col_groups = static_cast<int>((groups + a.col_blocks - 1) / a.col_blocks);
   a.rows = kActBwdMaxGroups / a.col_groups;
   a.passes = static_cast<int>((M + a.rows - 1) / a.rows);
-  const int64_t want = (3 * static_cast<int64_t>(sms)) / a.col_blocks;
+  const int64_t want = a.direct ? 1 : (3 * static_cast<int64_t>(sms)) / a.col_blocks;
   a.shares = static_cast<int>(want < 1 ? 1 : want < a.passes ? want : a.passes);
   return a;
+}
+
+// Partial sums of the bias gradient: none where one share sums all rows.
+static size_t act_bwd_ws(const ActBwdPlan& a, int64_t N) {
+  return a.shares > 1 ? static_cast<size_t>(a.shares) * static_cast<size_t>(N) * 4u : 0u;
 }
 
 int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
@@ -1617,7 +1628,7 @@ int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
   DeviceInfo* d;
   rc = device_info(&d);
   if (rc) return rc;
-  *bytes = static_cast<size_t>(act_bwd_plan(d->sms, M, N).shares) * static_cast<size_t>(N) * 4u;
+  *bytes = act_bwd_ws(act_bwd_plan(d->sms, M, N), N);
   return LTXFP8_OK;
 }
 
@@ -1645,11 +1656,12 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   rc = device_info(&d);
   if (rc) return rc;
   const ActBwdPlan pl = act_bwd_plan(d->sms, M, N);
-  if (dbias) {
-    if (!workspace || workspace_bytes < static_cast<size_t>(pl.shares) * static_cast<size_t>(N) * 4u)
+  if (dbias && !aligned(dbias, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: dbias must be 4-byte aligned", name);
+  const size_t need = dbias ? act_bwd_ws(pl, N) : 0;
+  if (need) {
+    if (!workspace || workspace_bytes < need)
       return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: the workspace is missing or too small", name);
-    if (!aligned(workspace, 16) || !aligned(dbias, 4))
-      return fail(LTXFP8_ERR_MISALIGNED, "%s: workspace must be 16-byte, dbias 4-byte aligned", name);
+    if (!aligned(workspace, 16)) return fail(LTXFP8_ERR_MISALIGNED, "%s: workspace must be 16-byte aligned", name);
   }
   ActBwdParams p;
   p.dy = static_cast<const __nv_bfloat16*>(dy);
@@ -1667,16 +1679,24 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   p.dzq = static_cast<uint8_t*>(dzq);
   p.dzs = dzs;
   p.dzs_ld = dzs_ld;
-  p.db_part = dbias ? static_cast<float*>(workspace) : nullptr;
+  p.db_part = need ? static_cast<float*>(workspace) : dbias;
   const dim3 grid(static_cast<unsigned>(pl.col_blocks), static_cast<unsigned>(pl.shares));
   const bool gelu = activation == LTXFP8_ACT_GELU_TANH;
-  auto kern = gelu ? act_backward_kernel<kActGeluTanh> : act_backward_kernel<kActSilu>;
-  cudaError_t e = allow_smem(kern, &d->act_bwd_ready[gelu], kActBwdSmemBytes);
-  if (e != cudaSuccess) return cuda_fail(e, "act_backward smem");
-  kern<<<grid, 256, kActBwdSmemBytes, s>>>(p);
-  e = cudaGetLastError();
+  cudaError_t e;
+  if (pl.direct) {
+    auto kern = gelu ? act_backward_kernel<kActGeluTanh, true> : act_backward_kernel<kActSilu, true>;
+    // (the joined rows' sums only)
+    kern<<<grid, 256, kActBwdMaxGroups * 512, s>>>(p);
+    e = cudaGetLastError();
+  } else {
+    auto kern = gelu ? act_backward_kernel<kActGeluTanh, false> : act_backward_kernel<kActSilu, false>;
+    e = allow_smem(kern, &d->act_bwd_ready[gelu], kActBwdSmemBytes);
+    if (e != cudaSuccess) return cuda_fail(e, "act_backward smem");
+    kern<<<grid, 256, kActBwdSmemBytes, s>>>(p);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return cuda_fail(e, "act_backward launch");
-  if (dbias) {
+  if (need) {
     e = launch_dependent(col_sum_kernel, static_cast<unsigned>((N + 31) / 32), kColSumWarps * 32, s, p.db_part,
                          pl.shares, static_cast<int>(N), dbias, true);
     if (e != cudaSuccess) return cuda_fail(e, "act_backward sum launch");

@@ -233,19 +233,23 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
   const int64_t row_groups = (p.M + kRows - 1) / kRows;
   const int passes = static_cast<int>((row_groups - blockIdx.x + gridDim.x - 1) / gridDim.x);
 
-  // Warp 0: fetch the rows of pass j, one copy a lane (row r of input i at (r * inputs + i)).
+  // Warp 0: fetch the rows of pass j (input i's row r at (i * kRows + r)), a copy per input where
+  // its rows are contiguous, else one per row: many small copies cost more than their bytes
+  // (256-byte rows one by one took 1.5 us a pass).
   auto load_pass = [&](int j) {
     const int64_t r0 = (blockIdx.x + static_cast<int64_t>(j) * gridDim.x) * kRows;
     const int rows = static_cast<int>(p.M - r0 < kRows ? p.M - r0 : kRows);
     uint64_t* bar = &full[j % p.stages];
     if (lane == 0) mbar_arrive_expect_tx(bar, row_bytes * rows * inputs);
     __syncwarp();
-    if (lane < rows * inputs) {
-      const int r = lane / inputs, i = lane - r * inputs;
-      const __nv_bfloat16* src = i == 0   ? p.dy + (r0 + r) * p.dy_ld
-                                 : i == 1 ? p.h + (r0 + r) * p.h_ld
-                                          : p.dh + (r0 + r) * p.dh_ld;
-      bulk_load(bar, ring + (j % p.stages) * stage_bytes + lane * row_bytes, src, row_bytes);
+    const int i = lane / kRows, r = lane - i * kRows;
+    if (i < inputs && r < rows) {
+      const __nv_bfloat16* base = i == 0 ? p.dy : i == 1 ? p.h : p.dh;
+      const int64_t ld = i == 0 ? p.dy_ld : i == 1 ? p.h_ld : p.dh_ld;
+      const bool whole = ld == p.H;
+      if (!whole || r == 0)
+        bulk_load(bar, ring + (j % p.stages) * stage_bytes + lane * row_bytes, base + (r0 + r) * ld,
+                  whole ? row_bytes * rows : row_bytes);
     }
   };
   if (threadIdx.x == 0) {
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
     const float rstd = rstd_next;
     rstd_next = row + row_step < p.M ? __ldg(p.rstd + row + row_step) : 0.0f;
     ok = mbar_wait(&full[j % p.stages], (j / p.stages) & 1u, kStNormLoad);
-    const uint8_t* src = ring + (j % p.stages) * stage_bytes + (warp / kWarps) * inputs * row_bytes;
+    const uint8_t* src = ring + (j % p.stages) * stage_bytes + (warp / kWarps) * row_bytes;
     Run16 vy[kChunks], vh[kChunks], vd[kChunks];
     float acc = 0.0f;
     const float2 r2 = make_float2(rstd, rstd);
@@ -289,8 +293,8 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
       const bool in = row_ok && col < p.H;
       const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(src) + col;
       vy[i] = in ? ld_run(v) : zero_run();
-      vh[i] = in ? ld_run(v + p.H) : zero_run();
-      vd[i] = (in && inputs == 3) ? ld_run(v + 2 * p.H) : zero_run();
+      vh[i] = in ? ld_run(v + kRows * p.H) : zero_run();
+      vd[i] = (in && inputs == 3) ? ld_run(v + 2 * kRows * p.H) : zero_run();
       float2 y[8], x[8], s = make_float2(0.0f, 0.0f);
       run_to_f2(vy[i], y);
       run_to_f2(vh[i], x);

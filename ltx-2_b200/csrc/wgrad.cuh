@@ -149,18 +149,19 @@ __global__ void __launch_bounds__(kWgThreads, 1)
   const bool leader = rank == 0;
   const int team = static_cast<int>(blockIdx.x) / kCtas, teams = static_cast<int>(gridDim.x) / kCtas;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kWgMaxStages; ++s) {
-      mbar_init(&raw_full[s], 1);
-      mbar_init(&raw_empty[s], kWgGroupWarps);
-      mbar_init(&g_full[s], 1);
-      mbar_init(&g_empty[s], 1);
-      mbar_init(&op_full[s], kXFp8 ? kWgGroupWarps * kCtas : 1);
-      mbar_init(&op_empty[s], 1);
+  if (threadIdx.x < kWgMaxStages) {
+    const int s = static_cast<int>(threadIdx.x);
+    mbar_init(&raw_full[s], 1);
+    mbar_init(&raw_empty[s], kWgGroupWarps);
+    mbar_init(&g_full[s], 1);
+    mbar_init(&g_empty[s], 1);
+    mbar_init(&op_full[s], kXFp8 ? kWgGroupWarps * kCtas : 1);
+    mbar_init(&op_empty[s], 1);
+    if (s == 0) {
+      mbar_init(acc_full, 1);
+      mbar_init(acc_empty, kWgExpandWarps * kCtas);
+      mbar_init(drain, 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, kWgExpandWarps * kCtas);
-    mbar_init(drain, 1);
     fence_mbarrier_init();
   }
   if (warp == 0 && lane == 0) {
