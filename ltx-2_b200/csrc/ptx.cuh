@@ -299,33 +299,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// The same, publishing this thread's earlier writes to the threads of the cluster that wait
-// on the barrier with mbar_wait_cluster.
+// The same, with its release at cluster scope.
 __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
-// mbar_wait with acquire semantics over the cluster (arrivals come from the peer CTA too).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, unsigned int code,
-                                                  unsigned long long limit_ns = kWaitLimitNs) {
-  unsigned long long t0 = 0;
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    const unsigned long long t = globaltimer_ns();
-    if (t0 == 0) t0 = t;
-    if (t - t0 > limit_ns) {
-      record_status(code);
-      return false;
-    }
-  }
 }
 
 // 2-D tile load into this CTA's shared memory whose completion is counted on the

@@ -3,6 +3,8 @@ from an 8-bit checkpoint, and the weight's transpose, against 64-bit evaluations
 (csrc/act_checkpoint.cuh, csrc/wgrad.cuh)."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -66,7 +68,7 @@ GRAD_ABS = 1.5 * 2.0 ** -18
 
 
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("M,N", [(1, 128), (2, 4096), (37, 384), (300, 1152), (1003, 2048), (40, 16384), (5000, 128)])
+@pytest.mark.parametrize("M,N", [(1, 128), (2, 4096), (37, 384), (64, 1152), (65, 256), (300, 1152), (1003, 2048), (40, 16384), (5000, 128)])
 def test_backward(cuda_device, M, N, act):
     from ltx_kernels.blockwise import ops
     zero = (M // 2,) if M > 2 else ()
@@ -96,9 +98,9 @@ def test_backward(cuda_device, M, N, act):
     amax = g.abs().amax(-1)
     assert ((ds.double() * 448 - amax).abs() <= amax * 2.0 ** -20 + (dy64.abs() * GRAD_ABS).view_as(g).amax(-1)
             + 2.0 ** -110).all()
-    # a thread adds its rows in turn (at most every 4th row of a share), a block joins 32 rows,
-    # the shares are summed in 8 chains
-    steps = M / 4 + 32 + 8 + M / 8 + 8
+    # a thread adds at most every second row of its share (M / 2 of a single share is at most 32),
+    # a block joins at most 32 rows, the shares (at most M / 2 of them) are summed in 32 chains
+    steps = M / 2 + 32 + M / 64 + 32
     assert_close(db, want.sum(0), (want.abs() * steps * U32 + dy64.abs() * GRAD_ABS).sum(0), "dbias")
 
 
@@ -122,6 +124,13 @@ def test_act_strided_empty_and_layouts(cuda_device):
     c = ops.act_quantize_save(big[:, 8:520].reshape(5, 10, 512), "silu")
     for i in range(4):
         assert torch.equal(a[i].float(), b[i].float()) and torch.equal(c[i].float(), b[i].float())
+    for M, N in ((300, 384), (130, 1152)):  # one column block, and two: rows fetched one by one
+        zq, zs = quant_rows(_z(M, N, 38).float())
+        zq, zs, wide = zq.to(cuda_device), mn_major(zs).to(cuda_device), grads(M, N + 40, 39).to(cuda_device)
+        dy = wide[:, 8:N + 8]
+        for x, y in zip(ops.act_backward(dy, zq, zs, "silu", quantize=True, dbias=True),
+                        ops.act_backward(dy.contiguous(), zq, zs, "silu", quantize=True, dbias=True)):
+            assert torch.equal(x.float(), y.float())
     dy = grads(50, 600, 37).to(cuda_device)
     d1 = ops.act_backward(dy[:, 3:515], a[2], a[3], "silu", quantize=True, dbias=True)
     d2 = ops.act_backward(dy[:, 3:515].contiguous(), a[2], a[3].t().contiguous(), "silu", quantize=True, dbias=True)
@@ -145,6 +154,32 @@ def _wgrad_tol(want, size, M):
     # fp32 accumulation, at most one rounding or truncation (2^-22 of the running size) per
     # 16-token step of the tensor core and per split, then alpha and the output's rounding
     return want.abs() * (UBF16 + 2 * U32) + (M / 16 + 70) * 2.0 ** -22 * size
+
+
+def test_wgrad_forms(cuda_device):
+    """One CTA and the pair of CTAs, with and without a split over the tokens, each with tokens,
+    rows and columns that end inside a tile."""
+    from ltx_kernels import _lib
+    from ltx_kernels.blockwise import ops
+    seen = set()
+    sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    for M, N, K in ((333, 48, 384), (5001, 144, 1152), (77, 2064, 1152), (333, 2064, 384), (1001, 528, 2176),
+                    (2001, 144, 896), (5001, 2064, 896)):
+        i = _lib.WgradPlanInfo()
+        assert _lib.load().ltxfp8_wgrad_plan_for_sms(M, N, K, sms, ctypes.byref(i)) == _lib.OK
+        seen.add((bool(i.pair), i.splits > 1))
+        xq, xs = quant_rows(tokens(M, K, 46).float())
+        g = grads(M, N, 47).to(cuda_device)
+        qd, sd = xq.to(cuda_device), mn_major(xs.to(cuda_device))
+        xb = (qd.float() * sd.repeat_interleave(128, 1)).to(torch.bfloat16)
+        want, size = _wgrad64(g, xb, 1.0)
+        for transposed in (False, True):
+            a = ops.wgrad_1x128(g, qd, sd, transposed=transposed)
+            b = ops.wgrad_bf16(g, xb, transposed=transposed)
+            a, b = (a.t(), b.t()) if transposed else (a, b)
+            assert_close(a, want, _wgrad_tol(want, size, M), f"{M, N, K}")
+            assert torch.equal(a, b)
+    assert len(seen) == 4, seen
 
 
 @pytest.mark.parametrize("M,N,K", [

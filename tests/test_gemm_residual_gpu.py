@@ -41,6 +41,8 @@ def _want(aq, asc, wq, wsc, b, r, act):
 @pytest.mark.parametrize("M,N,K", [
     (1, 128, 128), (1, 4096, 4096),    # single tokens: one tile, and split-K
     (7, 1024, 2048), (33, 384, 128), (129, 640, 1152),
+    (8, 256, 1152), (9, 128, 128), (16, 384, 2176), (16, 4096, 4096), (17, 256, 1152),  # the streaming kernel's ends
+    (12, 8192, 4224),                  # its widest weight passed
     (257, 4096, 512),                  # more than half of a wave of tiles
     (2100, 1152, 256),                 # several row tiles, ragged, N ends inside a tile
     (1280, 4096, 8192),                # the last rows split over K
@@ -63,7 +65,7 @@ def test_against_64_bits(cuda_device, M, N, K, act, res):
 def test_options(cuda_device):
     """No bias, no split, a strided or misaligned residual, and the residual updated in place."""
     from ltx_kernels.blockwise import ops
-    for M, N, K in ((70, 512, 4096), (700, 4096, 256)):
+    for M, N, K in ((3, 512, 1152), (13, 384, 640), (70, 512, 4096), (700, 4096, 256)):
         aq, asc, wq, wsc, b, r = _problem(M, N, K, cuda_device, seed=7)
         y, tol = _want(aq, asc, wq, wsc, None, r, None)
         assert_close(ops.gemm_residual(aq, asc, wq, wsc, residual=r), y, tol)

@@ -161,9 +161,9 @@ def test_backward(cuda_device, M, H, res, gain):
         assert dw is None
     else:
         assert dw.dtype == gain and dw.shape == (H,)
-        # a block adds at most M / 148 of its rows in turn, joins 8 row groups, and the at most
-        # 592 blocks are summed in 8 chains; each product carries two roundings of its own
-        steps = M / 148 + 1 + 8 + 592 / 8 + 8 + 2
+        # a block (at least one an SM) adds at most M / 148 of its rows in turn, joins 8 row groups,
+        # and the at most 296 blocks are summed in 32 chains; each product has two roundings of its own
+        steps = M / 148 + 1 + 8 + 296 / 32 + 1 + 32 + 2
         tol = steps * U32 * dwabs + (dw64.abs() * UBF16 if gain == torch.bfloat16 else 0)
         assert_close(dw, dw64, tol, "dw")
 
