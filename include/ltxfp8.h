@@ -41,6 +41,8 @@ extern "C" {
 #define LTXFP8_QUANT_FINITE 2 /* scale = max(amax, 448 * 2^-126) / 448, code = e4m3(x / scale), within 1 ulp: an all-zero
                                  group gets zero codes (the modes above give NaN there).  ltxfp8_quantize_1x128 only;
                                  the residual-path operators at the end of this file always quantise this way */
+#define LTXFP8_QUANT_ZEROS 4  /* added to _TORCH or _TRITON in ltxfp8_quantize_1x128: the same codes and scales, but a
+                                 group whose s overflows (all zeros) gets zero codes and scale 0 instead of NaN */
 
 /* Input dtypes for ltxfp8_quantize_weight_128x128. */
 #define LTXFP8_DTYPE_F32 0
@@ -58,7 +60,7 @@ const char* ltxfp8_last_error(void);
  *   x      bf16 [M, K], row stride x_ld elements (x_ld >= K, x_ld % 8 == 0)
  *   q      e4m3 [M, K], row stride q_ld bytes (q_ld % 8 == 0)
  *   sfa    fp32, element (m, kb) at sfa[kb * sfa_ld + m], sfa_ld >= M
- *   K % 128 == 0.  flags: LTXFP8_QUANT_TORCH, LTXFP8_QUANT_TRITON or LTXFP8_QUANT_FINITE.
+ *   K % 128 == 0.  flags: LTXFP8_QUANT_TORCH or _TRITON (with or without _ZEROS), or _FINITE.
  * Replaces the Triton op blockwise::quantize with use_gelu=False
  * (ltx-kernels/src/ltx_kernels/blockwise/triton_ops.py:128-151, kernel :102-126)
  * and blockwise_quantize_torch (functional.py:138-144).
@@ -83,6 +85,14 @@ int ltxfp8_quantize_weight_128x128(const void* w, int dtype, int64_t N, int64_t 
  */
 int ltxfp8_quantize_weight_128x128_scaled(const void* w, int dtype, int64_t N, int64_t K, float scale_max, void* q,
                                           float* sfb, void* stream);
+
+/*
+ * As ltxfp8_quantize_weight_128x128 (the same codes and scales), but a block whose s
+ * overflows (all zeros, as in a zero-initialised weight) gets zero codes and scale 0
+ * instead of NaN.  No reference counterpart (master weights are quantised per training step).
+ */
+int ltxfp8_quantize_weight_128x128_finite(const void* w, int dtype, int64_t N, int64_t K, void* q, float* sfb,
+                                          void* stream);
 
 /*
  * FP6 packing of e4m3 codes [m, n] (n % 8 == 0) into [m, n * 3 / 4] bytes: each code

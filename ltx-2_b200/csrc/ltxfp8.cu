@@ -547,7 +547,9 @@ const char* ltxfp8_last_error(void) { return t_last_error.c_str(); }
 int ltxfp8_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, void* q, int64_t q_ld, float* sfa,
                           int64_t sfa_ld, int flags, void* stream) {
   if (M < 0 || K <= 0 || K % 128 != 0) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize: need K %% 128 == 0, K > 0, M >= 0 (M=%lld K=%lld)", (long long)M, (long long)K);
-  if (flags != LTXFP8_QUANT_TORCH && flags != LTXFP8_QUANT_TRITON && flags != LTXFP8_QUANT_FINITE)
+  const int mode = flags & ~LTXFP8_QUANT_ZEROS;
+  const bool zeros = (flags & LTXFP8_QUANT_ZEROS) != 0;
+  if (mode != LTXFP8_QUANT_TORCH && mode != LTXFP8_QUANT_TRITON && flags != LTXFP8_QUANT_FINITE)
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: unknown mode %d", flags);
   if (M == 0) return LTXFP8_OK;
   if (!x || !q || !sfa) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize: null pointer");
@@ -565,57 +567,50 @@ int ltxfp8_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, voi
   auto s = static_cast<cudaStream_t>(stream);
   const auto* xb = static_cast<const __nv_bfloat16*>(x);
   auto* qb = static_cast<uint8_t*>(q);
-  if (flags == LTXFP8_QUANT_TRITON)
-    quant_act_1x128_kernel<kQuantTriton><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
-  else if (flags == LTXFP8_QUANT_FINITE)
-    quant_act_1x128_kernel<kQuantFinite><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
-  else
-    quant_act_1x128_kernel<kQuantTorch><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
+  auto kern = mode == LTXFP8_QUANT_FINITE ? quant_act_1x128_kernel<kQuantFinite>
+              : mode == LTXFP8_QUANT_TRITON
+                  ? (zeros ? quant_act_1x128_kernel<kQuantTriton, true> : quant_act_1x128_kernel<kQuantTriton>)
+                  : (zeros ? quant_act_1x128_kernel<kQuantTorch, true> : quant_act_1x128_kernel<kQuantTorch>);
+  kern<<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantize launch");
   return LTXFP8_OK;
 }
 
-int ltxfp8_quantize_weight_128x128(const void* w, int dtype, int64_t N, int64_t K, void* q, float* sfb,
-                                   void* stream) {
+static int quant_weight(const char* name, const void* w, int dtype, int64_t N, int64_t K, float scale_max, bool zeros,
+                        void* q, float* sfb, void* stream) {
   if (N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0)
-    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize_weight: N and K must be positive multiples of 128 (N=%lld K=%lld)", (long long)N, (long long)K);
-  if (dtype < LTXFP8_DTYPE_F32 || dtype > LTXFP8_DTYPE_F16) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize_weight: unknown dtype %d", dtype);
-  if (!w || !q || !sfb) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize_weight: null pointer");
-  if (!aligned(w, 16) || !aligned(q, 16) || !aligned(sfb, 4)) return fail(LTXFP8_ERR_MISALIGNED, "quantize_weight: w and q must be 16-byte aligned");
-  if (N / 128 > 65535) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize_weight: N too large");
+    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: N and K must be positive multiples of 128 (N=%lld K=%lld)", name, (long long)N, (long long)K);
+  if (dtype < LTXFP8_DTYPE_F32 || dtype > LTXFP8_DTYPE_F16) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", name, dtype);
+  if (!w || !q || !sfb) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  if (!aligned(w, 16) || !aligned(q, 16) || !aligned(sfb, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: w and q must be 16-byte aligned", name);
+  if (N / 128 > 65535) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "%s: N too large", name);
   DeviceInfo* d;
   int rc = device_info(&d);
   if (rc) return rc;
   dim3 grid(static_cast<unsigned>(K / 128), static_cast<unsigned>(N / 128));
-  quant_weight_128x128_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(w, dtype, K, K / 128,
-                                                                                    static_cast<uint8_t*>(q), sfb,
-                                                                                    448.0f);
+  quant_weight_128x128_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      w, dtype, K, K / 128, static_cast<uint8_t*>(q), sfb, scale_max, zeros);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantize_weight launch");
   return LTXFP8_OK;
+}
+
+int ltxfp8_quantize_weight_128x128(const void* w, int dtype, int64_t N, int64_t K, void* q, float* sfb,
+                                   void* stream) {
+  return quant_weight("quantize_weight", w, dtype, N, K, 448.0f, false, q, sfb, stream);
 }
 
 int ltxfp8_quantize_weight_128x128_scaled(const void* w, int dtype, int64_t N, int64_t K, float scale_max, void* q,
                                           float* sfb, void* stream) {
   if (!(scale_max > 0.0f) || !(scale_max <= 448.0f))
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize_weight_scaled: scale_max must be in (0, 448]");
-  if (N <= 0 || K <= 0 || N % 128 != 0 || K % 128 != 0)
-    return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize_weight_scaled: N and K must be positive multiples of 128 (N=%lld K=%lld)", (long long)N, (long long)K);
-  if (dtype < LTXFP8_DTYPE_F32 || dtype > LTXFP8_DTYPE_F16) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize_weight_scaled: unknown dtype %d", dtype);
-  if (!w || !q || !sfb) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "quantize_weight_scaled: null pointer");
-  if (!aligned(w, 16) || !aligned(q, 16) || !aligned(sfb, 4)) return fail(LTXFP8_ERR_MISALIGNED, "quantize_weight_scaled: w and q must be 16-byte aligned");
-  if (N / 128 > 65535) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "quantize_weight_scaled: N too large");
-  DeviceInfo* d;
-  int rc = device_info(&d);
-  if (rc) return rc;
-  dim3 grid(static_cast<unsigned>(K / 128), static_cast<unsigned>(N / 128));
-  quant_weight_128x128_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(w, dtype, K, K / 128,
-                                                                                    static_cast<uint8_t*>(q), sfb,
-                                                                                    scale_max);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "quantize_weight_scaled launch");
-  return LTXFP8_OK;
+  return quant_weight("quantize_weight_scaled", w, dtype, N, K, scale_max, false, q, sfb, stream);
+}
+
+int ltxfp8_quantize_weight_128x128_finite(const void* w, int dtype, int64_t N, int64_t K, void* q, float* sfb,
+                                          void* stream) {
+  return quant_weight("quantize_weight_finite", w, dtype, N, K, 448.0f, true, q, sfb, stream);
 }
 
 static int fp6_launch(bool pack, const void* x, int64_t m, int64_t n, void* out, void* stream) {

@@ -43,7 +43,8 @@ __device__ __forceinline__ void group_scale(float amax, float& s, float& inv) {
 // sfa[kb * sfa_ld + m] = 1 / s.  Block = 16 rows x kQuantGroupsPerThread groups;
 // each half-warp owns one row-group of 128 values (8 per lane, one 16 B load).
 // Replaces _block_quant_kernel (ltx-kernels/src/ltx_kernels/blockwise/triton_ops.py:102-126).
-template <int kMode>
+// kZeros: a group whose s overflows (all zeros, or below 2^-119) gets zero codes and scale 0.
+template <int kMode, bool kZeros = false>
 __global__ void __launch_bounds__(256) quant_act_1x128_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_ld,
                                                               int64_t M, int64_t KB, uint8_t* __restrict__ q,
                                                               int64_t q_ld, float* __restrict__ sfa,
@@ -80,6 +81,7 @@ __global__ void __launch_bounds__(256) quant_act_1x128_kernel(const __nv_bfloat1
     }
     float s, inv;
     group_scale<kMode>(amax, s, inv);
+    if (kZeros && isinf(s)) s = inv = 0.0f;
     // A finite scale keeps every |x * s| <= 448, where the saturating hardware
     // conversion equals torch's; only non-finite scales need torch's overflow-to-NaN
     // patch.  The Triton kernel converts with the saturating instruction throughout.
@@ -172,8 +174,9 @@ __global__ void __launch_bounds__(256) gelu_tanh_quant_kernel(const __nv_bfloat1
 // consecutive values f of one row of the block.  Block abs-max (NaN-propagating,
 // as torch's abs().max()), s = (1/amax)*scale_max, codes e4m3(f*s) with torch's
 // conversion to `qrow` (this thread's 64 bytes), scale 1/s to *scale by thread 0.
+// zeros: a block whose s overflows (all zeros, or below 2^-119) gets zero codes and scale 0.
 __device__ __forceinline__ void quant_block_128x128_store(const float (&f)[64], float* red, uint8_t* qrow,
-                                                          float* scale, float scale_max = 448.0f) {
+                                                          float* scale, float scale_max = 448.0f, bool zeros = false) {
   const int t = threadIdx.x;
   float amax = 0.0f;
 #pragma unroll
@@ -185,7 +188,9 @@ __device__ __forceinline__ void quant_block_128x128_store(const float (&f)[64], 
   amax = red[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) amax = fmax_nan(amax, red[i]);
-  const float s = __fmul_rn(__frcp_rn(amax), scale_max);
+  float s = __fmul_rn(__frcp_rn(amax), scale_max);
+  zeros = zeros && isinf(s);
+  if (zeros) s = 0.0f;
   uint32_t words[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -196,7 +201,7 @@ __device__ __forceinline__ void quant_block_128x128_store(const float (&f)[64], 
   uint4* dst = reinterpret_cast<uint4*>(qrow);
 #pragma unroll
   for (int i = 0; i < 4; ++i) dst[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
-  if (t == 0) *scale = __frcp_rn(s);
+  if (t == 0) *scale = zeros ? 0.0f : __frcp_rn(s);
 }
 
 // Weight quant over 128x128 blocks: one block of 256 threads per (kb, nb); each
@@ -205,7 +210,8 @@ __device__ __forceinline__ void quant_block_128x128_store(const float (&f)[64], 
 // in_dtype: 0 = fp32, 1 = bf16, 2 = fp16.
 __global__ void __launch_bounds__(256) quant_weight_128x128_kernel(const void* __restrict__ w, int in_dtype, int64_t K,
                                                                    int64_t KB, uint8_t* __restrict__ q,
-                                                                   float* __restrict__ sfb, float scale_max) {
+                                                                   float* __restrict__ sfb, float scale_max,
+                                                                   bool zeros) {
   __shared__ float red[8];
   const int t = threadIdx.x;
   const int64_t kb = blockIdx.x, nb = blockIdx.y;
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(256) quant_weight_128x128_kernel(const void* _
       }
     }
   }
-  quant_block_128x128_store(f, red, q + r * K + c0, sfb + nb * KB + kb, scale_max);
+  quant_block_128x128_store(f, red, q + r * K + c0, sfb + nb * KB + kb, scale_max, zeros);
 }
 
 // Dequant: out[m, k] = bf16(float(q[m, k]) * scales[m * rs + (k / 128) * cs]).

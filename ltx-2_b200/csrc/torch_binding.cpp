@@ -4,7 +4,7 @@
 //
 // These operators are called per token step and per layer, where the host's time for a call
 // matters: building four output tensors, the checks and a 16-argument ctypes call from Python
-// take 17-28 us, most of it more than the kernel; here a call takes 7-11 us.  The functions
+// take 17-28 us, most of it more than the kernel; here a call takes 5-13 us.  The functions
 // take positional arguments only; the Python wrappers in ltx_kernels/blockwise/ops.py name
 // and document them.
 #include <Python.h>
@@ -15,7 +15,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <string>
 
@@ -401,6 +403,24 @@ PyObject* wgrad_bf16(PyObject* const* a) {
   return wgrad_call(name, dev, g, xr.ptr(), xr.M, xr.K, xr.ld, nullptr, 0, double_arg(a[2]), bool_arg(a[3]));
 }
 
+// (name, leaves): refuse a capture in which autograd would reach a leaf's gradient node that was
+// made on the default stream and is still alive.
+PyObject* check_capture(PyObject* const* a) {
+  const char* name = PyUnicode_AsUTF8(a[0]);
+  if (!name) throw python_error();
+  TORCH_CHECK_TYPE(PyList_Check(a[1]), name, ": expected a list of tensors");
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[1]); ++i) {
+    const Tensor t = tensor_arg(name, "a leaf", PyList_GET_ITEM(a[1], i));
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node || !t.is_cuda()) continue;
+    const auto s = node->stream();
+    TORCH_CHECK(!s || c10::cuda::CUDAStream(*s) != c10::cuda::getDefaultCUDAStream(t.device().index()), name,
+                ": a leaf's gradient node from an earlier eager result on the default stream is still alive; release "
+                "that result (or compute it on a side stream) before capturing");
+  }
+  Py_RETURN_NONE;
+}
+
 // (check): the Python function that raises for a C-ABI return code.
 PyObject* set_check(PyObject* const* a) {
   Py_INCREF(a[0]);
@@ -430,7 +450,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef kMethods[] = {
     LTXFP8_ENTRY(rms_norm_quantize, 5), LTXFP8_ENTRY(rms_norm_backward, 5), LTXFP8_ENTRY(gemm_residual, 9),
     LTXFP8_ENTRY(act_quantize_save, 3), LTXFP8_ENTRY(act_backward, 6),      LTXFP8_ENTRY(wgrad_1x128, 5),
-    LTXFP8_ENTRY(wgrad_bf16, 4),        LTXFP8_ENTRY(set_check, 1),         {nullptr, nullptr, 0, nullptr}};
+    LTXFP8_ENTRY(wgrad_bf16, 4),        LTXFP8_ENTRY(check_capture, 2),
+    LTXFP8_ENTRY(set_check, 1),         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ltxfp8_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

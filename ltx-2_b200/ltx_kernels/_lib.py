@@ -25,6 +25,7 @@ ERR_DEVICE_STATUS = -6
 QUANT_TORCH = 0
 QUANT_TRITON = 1
 QUANT_FINITE = 2  # scale = amax / 448, all-zero groups quantise to zeros
+QUANT_ZEROS = 4  # added to QUANT_TORCH / QUANT_TRITON: all-zero groups quantise to zeros
 
 GELU_NONE = 0
 GELU_TANH = 1       # torch's CUDA GELU-tanh formula (bit-identical bf16 results)
@@ -111,6 +112,7 @@ SIGNATURES = {
     "ltxfp8_rms_norm_split_rope": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64,
                                           _vp, _vp, _i32, _vp]),
     "ltxfp8_lora_fuse_weight": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "ltxfp8_quantize_weight_128x128_finite": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
     "ltxfp8_quantize_weight_128x128_scaled": (_i32, [_vp, _i32, _i64, _i64, _f32, _vp, _vp, _vp]),
     "ltxfp8_fp6_pack": (_i32, [_vp, _i64, _i64, _vp, _vp]),
     "ltxfp8_fp6_unpack": (_i32, [_vp, _i64, _i64, _vp, _vp]),

@@ -21,6 +21,7 @@ from typing import Optional, Tuple, Union
 import torch
 import torch.nn as nn
 
+from .. import _lib as L
 from . import ops
 from .functional import blockwise_quantize_triton, quant_mode_code
 from .linear import BlockwiseFP8Linear
@@ -106,8 +107,9 @@ class BlockwiseFP8LoRALinear(BlockwiseFP8Linear):
     """BlockwiseFP8Linear plus a runtime LoRA ``alpha * B (A x)`` (bf16 A ``[r, in]``, B ``[out, r]``).
 
     The factors are frozen by default.  Where gradients are enabled and the input, a factor or
-    the bias requires one, the forward is :func:`training.fp8_linear_train`: differentiable,
-    keeping the input in 8 bits (``layer.lora_A.requires_grad_()`` starts a LoRA fine-tune)."""
+    the bias requires one, the forward is :func:`training.fp8_linear_train`: the same output,
+    differentiable, keeping the input in 8 bits (``layer.lora_A.requires_grad_()`` starts a LoRA
+    fine-tune); only an all-zero 1x128 group of the input, NaN otherwise, counts as zeros there."""
 
     def __init__(self, in_features: int, out_features: int, rank: int, alpha: float = 1.0, bias: bool = True,
                  device=None, dtype=None):
@@ -126,5 +128,6 @@ class BlockwiseFP8LoRALinear(BlockwiseFP8Linear):
                                         or (self.bias is not None and self.bias.requires_grad)):
             from .training import fp8_linear_train
             return fp8_linear_train(x, (self.weight, self.weight_scale), self.bias,
-                                    lora=(self.lora_A, self.lora_B, self.alpha))
+                                    lora=(self.lora_A, self.lora_B, self.alpha),
+                                    quant_mode=quant_mode_code() | L.QUANT_ZEROS)
         return fp8_linear(x, self.weight, self.weight_scale, self.bias, lora=(self.lora_A, self.lora_B, self.alpha))

@@ -107,20 +107,28 @@ def quantize_1x128(x: torch.Tensor, mode: int = L.QUANT_TORCH) -> Tuple[torch.Te
     return q, s
 
 
-def quantize_weight_128x128(w: torch.Tensor, scale_max: float = 448.0) -> Tuple[torch.Tensor, torch.Tensor]:
-    """W [N, K] (fp32/bf16/fp16) -> (e4m3 [N, K], fp32 scales [N/128, K/128]); s = (1/amax)*scale_max."""
+def quantize_weight_128x128(w: torch.Tensor, scale_max: float = 448.0, *,
+                            finite: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """W [N, K] (fp32/bf16/fp16) -> (e4m3 [N, K], fp32 scales [N/128, K/128]); s = (1/amax)*scale_max.
+
+    ``finite`` (scale_max 448): an all-zero block gets zero codes and scale 0 instead of NaN."""
     _require_cuda("quantize_weight_128x128", w)
     dt = {torch.float32: L.DTYPE_F32, torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}.get(w.dtype)
     if dt is None:
         raise RuntimeError(f"quantize_weight_128x128: unsupported dtype {w.dtype}")
     if w.dim() != 2:
         raise RuntimeError("quantize_weight_128x128 expects a 2-D weight")
+    if finite and scale_max != 448.0:
+        raise RuntimeError("quantize_weight_128x128: finite needs scale_max 448")
     w = w.contiguous()
     N, K = w.shape
     q = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=w.device)
     s = torch.empty((N // 128, K // 128), dtype=torch.float32, device=w.device)
     with _DeviceGuard(w):
-        if scale_max == 448.0:
+        if finite:
+            L.check(L.load().ltxfp8_quantize_weight_128x128_finite(w.data_ptr(), dt, N, K, q.data_ptr(), s.data_ptr(),
+                                                                   _stream(w)))
+        elif scale_max == 448.0:
             L.check(L.load().ltxfp8_quantize_weight_128x128(w.data_ptr(), dt, N, K, q.data_ptr(), s.data_ptr(),
                                                              _stream(w)))
         else:

@@ -41,8 +41,27 @@ def _fp8_weight(weight: Weight, name: str) -> Tuple[torch.Tensor, torch.Tensor, 
         return q, s, None
     if weight.dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError(f"{name}: a master weight must be fp32 or bf16, got {weight.dtype}")
-    q, s = ops.quantize_weight_128x128(weight.detach())
+    q, s = ops.quantize_weight_128x128(weight.detach(), finite=True)
     return q, s, weight
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """[..., width] as [M, width] with 16-byte aligned rows (a copy only where it has none: an
+    expanded or oddly sliced tensor)."""
+    t = t.reshape(-1, width)
+    if t.shape[0] and (t.stride(1) != 1 or t.data_ptr() % 16
+                       or (t.shape[0] > 1 and (t.stride(0) < width or t.stride(0) % 8))):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _check_capture(name: str, *leaves: Optional[torch.Tensor]) -> None:
+    """Refuse, while a CUDA graph is captured, leaves whose gradient node was made on the default
+    stream and is still alive (an earlier eager result that has not been released): autograd
+    would run that node on the default stream, which a capture forbids, and the error ends the
+    process from its backward thread."""
+    if torch.cuda.is_current_stream_capturing():
+        L.binding().check_capture(name, [t for t in leaves if t is not None and t.is_leaf and t.requires_grad])
 
 
 def _column_sum(g: torch.Tensor) -> torch.Tensor:
@@ -57,15 +76,16 @@ def _dgrad(g: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, **lora) -> tor
 
 
 def _bf16_grad(g: torch.Tensor, width: int) -> torch.Tensor:
-    return g.to(torch.bfloat16).reshape(-1, width)
+    return _rows(g.to(torch.bfloat16), width)
 
 
 class _LinearTrain(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, master, bias, lora_a, lora_b, residual, w_q, w_s, alpha):
+    def forward(ctx, x, master, bias, lora_a, lora_b, residual, w_q, w_s, alpha, quant_mode):
+        _check_capture("fp8_linear_train", x, master, bias, lora_a, lora_b, residual)
         K, N = x.shape[-1], w_q.shape[0]
-        x2 = x.reshape(-1, K)
-        q, s = ops.quantize_1x128(x2, L.QUANT_FINITE)
+        x2 = _rows(x, K)
+        q, s = ops.quantize_1x128(x2, quant_mode)
         ax = a = b = None
         if lora_a is not None:
             a, b = lora_a.to(torch.bfloat16), lora_b.to(torch.bfloat16)
@@ -76,7 +96,11 @@ class _LinearTrain(torch.autograd.Function):
         else:
             y = ops.gemm_residual(q, s, w_q, w_s, bias,
                                   residual=None if residual is None else residual.reshape(-1, N))
-        ctx.save_for_backward(q, s, w_q, w_s, ax, a, b)
+        # Only what the wanted gradients read: the codes for the weight or A, x A^T for B.
+        need_x, need_w, _, need_a, need_b = ctx.needs_input_grad[:5]
+        if not (need_w or need_a):
+            q = s = None
+        ctx.save_for_backward(q, s, w_q, w_s, ax if need_b else None, a, b)
         ctx.alpha = alpha
         ctx.x_meta = (x.shape, x.dtype)
         ctx.master_dtype = None if master is None else master.dtype
@@ -110,7 +134,7 @@ class _LinearTrain(torch.autograd.Function):
             db = ops.wgrad_bf16(ax, g, alpha=ctx.alpha, transposed=True).to(ctx.lora_dtypes[1])
         if need_r:
             dr = g.view(ctx.residual_shape)
-        return dx, dw, dbias, da, db, dr, None, None, None
+        return dx, dw, dbias, da, db, dr, None, None, None, None
 
 
 def _check_x(x: torch.Tensor, K: int, name: str) -> None:
@@ -127,7 +151,7 @@ def _check_bias(bias: Optional[torch.Tensor], N: int, name: str) -> None:
 
 def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tensor] = None, *,
                      lora: Optional[Tuple[torch.Tensor, torch.Tensor, float]] = None,
-                     residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     residual: Optional[torch.Tensor] = None, quant_mode: int = L.QUANT_FINITE) -> torch.Tensor:
     """Differentiable blockwise-FP8 linear, ``x W^T + bias [+ alpha (x A^T) B^T] [+ residual]``.
 
     ``x`` bf16 ``[..., K]``.  ``weight`` is a frozen ``(e4m3 [N, K], fp32 scales [N/128, K/128])``
@@ -136,9 +160,10 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
     alpha)``, r a multiple of 16 up to 256, used in bf16.  ``residual`` bf16 of the output's shape,
     added in the GEMM's epilogue (after the LoRA term when there is one).
 
-    What the backward pass keeps of ``x`` is its e4m3 codes and scales (``x~``), and with LoRA
-    ``x A^T``; the weight is not copied.  The gradient of ``x`` is a blockwise-FP8 GEMM of the
-    quantised output gradient."""
+    What the backward pass keeps of ``x`` is its e4m3 codes and scales (``x~``, where the weight
+    or A wants a gradient), and with LoRA ``x A^T``; the weight is not copied.  The gradient of
+    ``x`` is a blockwise-FP8 GEMM of the quantised output gradient.  ``quant_mode``: of ``x``, as
+    ``ops.quantize_1x128`` takes it."""
     name = "fp8_linear_train"
     shape = weight[0].shape if isinstance(weight, (tuple, list)) else weight.shape
     if len(shape) != 2:
@@ -158,21 +183,29 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
         if residual.shape[:-1] != x.shape[:-1]:
             raise RuntimeError(f"{name}: residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
     w_q, w_s, master = _fp8_weight(weight, name)
-    return _LinearTrain.apply(x, master, bias, la, lb, residual, w_q, w_s, float(alpha))
+    return _LinearTrain.apply(x, master, bias, la, lb, residual, w_q, w_s, float(alpha),
+                              quant_mode)
 
 
 class _PreNormFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, norm_weight, m1, b1, m2, b2, w1, s1, w2, s2, activation, eps, train):
+        _check_capture("pre_norm_feed_forward", x, residual, norm_weight, m1, b1, m2, b2)
         K = x.shape[-1]
         x2 = x.reshape(-1, K)
         r2 = None if residual is None else residual.reshape(-1, K)
         nq, ns, h, rstd = ops.rms_norm_quantize(x2, norm_weight, r2, eps=eps)
         z = ops.gemm(nq, ns, w1, s1, b1)
-        yq, ys, zq, zs = ops.act_quantize_save(z, activation, save=train)
+        # Only what the wanted gradients read: y's codes for W2, z's for all that lies below the
+        # activation, the normalised input's for W1, h and rstd for the norm and its inputs.
+        need_x, need_r, need_nw, need_w1, need_b1, need_w2, _ = ctx.needs_input_grad[:7] if train else (False,) * 7
+        below = need_x or need_r or need_nw
+        yq, ys, zq, zs = ops.act_quantize_save(z, activation, save=below or need_w1 or need_b1)
         out = ops.gemm_residual(yq, ys, w2, s2, b2, residual=h)
         if train:
-            ctx.save_for_backward(nq, ns, h, rstd, zq, zs, yq, ys, norm_weight, w1, s1, w2, s2)
+            keep = lambda want, *ts: ts if want else (None,) * len(ts)  # noqa: E731
+            ctx.save_for_backward(*keep(need_w1, nq, ns), *keep(below, h, rstd), zq, zs, *keep(need_w2, yq, ys),
+                                  norm_weight, w1, s1, w2, s2)
         ctx.activation = activation
         ctx.shape = x.shape
         ctx.master_dtypes = tuple(None if m is None else m.dtype for m in (m1, m2))
@@ -215,8 +248,9 @@ def pre_norm_feed_forward(x: torch.Tensor, w1: Weight, w2: Weight, *, residual: 
     ``(e4m3, scales)`` pair or a bf16 / fp32 master weight that gets a gradient; ``norm_weight``
     fp32 or bf16 ``[d]``; ``b1``, ``b2`` fp32; ``activation`` ``"gelu_tanh"`` or ``"silu"``.
     Differentiable in x, residual, norm_weight, master weights and biases.  The backward pass
-    keeps h in bf16 and the normalised input, the activation's input and its output in 8 bits;
-    without gradients nothing is kept and the activation's input is not quantised."""
+    keeps h in bf16, the activation's input in 8 bits and, for the gradients of w1 and w2, the
+    normalised input and the activation's output in 8 bits; without gradients nothing is kept
+    and the activation's input is not quantised."""
     name = "pre_norm_feed_forward"
     sh1, sh2 = (w[0].shape if isinstance(w, (tuple, list)) else w.shape for w in (w1, w2))
     if len(sh1) != 2 or tuple(sh2) != (sh1[1], sh1[0]):

@@ -20,7 +20,7 @@ def test_binding_is_built_and_complete():
     L, _ = _lib()
     b = L.binding()
     for f in ("rms_norm_quantize", "rms_norm_backward", "gemm_residual", "act_quantize_save", "act_backward",
-              "wgrad_1x128", "wgrad_bf16"):
+              "wgrad_1x128", "wgrad_bf16", "check_capture"):
         assert callable(getattr(b, f))
     with pytest.raises(TypeError, match="positional"):
         b.act_quantize_save()
@@ -137,12 +137,30 @@ def test_in_place_needs_contiguous_rows():
 
 def test_quantize_modes():
     L, lib = _lib()
-    for mode, ok in ((L.QUANT_FINITE, True), (3, False)):
+    for mode, ok in ((L.QUANT_FINITE, True), (3, False), (L.QUANT_TORCH | L.QUANT_ZEROS, True),
+                     (L.QUANT_TRITON | L.QUANT_ZEROS, True), (L.QUANT_FINITE | L.QUANT_ZEROS, False), (8, False),
+                     (-1, False)):
         rc = lib.ltxfp8_quantize_1x128(16, 0, 128, 128, 16, 128, 16, 0, mode, None)
         assert (rc == L.OK) == ok
     # the reference's producers keep their two arithmetics
     assert lib.ltxfp8_gated_attention(16, 16, 1, 4, 256, 2, 16, 16, 4, None, L.QUANT_FINITE, None) \
         == L.ERR_INVALID_ARGUMENT
+
+
+    w = lib.ltxfp8_quantize_weight_128x128_finite
+    assert w(P, 0, 100, 128, P, P, None) == L.ERR_UNSUPPORTED_SHAPE and w(P, 3, 128, 128, P, P, None) == L.ERR_INVALID_ARGUMENT
+    assert w(None, 0, 128, 128, P, P, None) == L.ERR_INVALID_ARGUMENT and w(P + 4, 0, 128, 128, P, P, None) == L.ERR_MISALIGNED
+
+
+def test_check_capture():
+    L, _ = _lib()
+    t = torch.zeros(3, requires_grad=True)
+    y = t * 2
+    assert L.binding().check_capture("f", [t]) is None and y.requires_grad  # a host leaf has no stream
+    with pytest.raises(TypeError, match="f"):
+        L.binding().check_capture("f", [1])
+    with pytest.raises(TypeError, match="list"):
+        L.binding().check_capture("f", t)
 
 
 def test_host_tensors_and_wrong_types_are_refused():
