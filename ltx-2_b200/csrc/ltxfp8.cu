@@ -1588,19 +1588,19 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
 
 // Blocks of the activation's backward: column blocks of up to 4096 columns, evenly divided,
 // times row shares that make up what is resident at once (three blocks an SM).
-// Up to 64 rows the blocks are one group wide and take all rows, 32 at a time: one launch, and
-// the bias gradient needs no partial sums.
+// A few rows (`direct`): blocks one group wide that take all rows, 32 at a time, straight from
+// memory: one launch, and the bias gradient needs no partial sums.  Measured, direct / shares, with
+// the bias gradient: 6 x 4096 3.7 / 4.7 us, 64 x 640 4.2 / 4.7, 64 x 16384 4.7 / 7.8, 128 x 640
+// 5.8 / 4.8, 128 x 16384 6.3 / 10.4; without it: 6 x 4096 2.7 / 3.2, 33 x 4096 3.7 / 3.2.
 struct ActBwdPlan {
   bool direct;
   int col_groups, col_blocks, rows, passes, shares;
 };
 
-constexpr int64_t kActBwdDirectRows = 64;
-
-static ActBwdPlan act_bwd_plan(int sms, int64_t M, int64_t N) {
+static ActBwdPlan act_bwd_plan(int sms, int64_t M, int64_t N, bool dbias) {
   ActBwdPlan a;
   const int64_t groups = N / 128;
-  a.direct = M <= kActBwdDirectRows;
+  a.direct = M <= (dbias ? 64 : 32);
   a.col_blocks = static_cast<int>(a.direct ? groups : (groups + kActBwdMaxGroups - 1) / kActBwdMaxGroups);
   a.col_groups = static_cast<int>((groups + a.col_blocks - 1) / a.col_blocks);
   a.rows = kActBwdMaxGroups / a.col_groups;
@@ -1623,7 +1623,7 @@ int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes) {
   DeviceInfo* d;
   rc = device_info(&d);
   if (rc) return rc;
-  *bytes = act_bwd_ws(act_bwd_plan(d->sms, M, N), N);
+  *bytes = act_bwd_ws(act_bwd_plan(d->sms, M, N, true), N);
   return LTXFP8_OK;
 }
 
@@ -1650,7 +1650,7 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   DeviceInfo* d;
   rc = device_info(&d);
   if (rc) return rc;
-  const ActBwdPlan pl = act_bwd_plan(d->sms, M, N);
+  const ActBwdPlan pl = act_bwd_plan(d->sms, M, N, dbias != nullptr);
   if (dbias && !aligned(dbias, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: dbias must be 4-byte aligned", name);
   const size_t need = dbias ? act_bwd_ws(pl, N) : 0;
   if (need) {
@@ -1680,8 +1680,7 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   cudaError_t e;
   if (pl.direct) {
     auto kern = gelu ? act_backward_kernel<kActGeluTanh, true> : act_backward_kernel<kActSilu, true>;
-    // (the joined rows' sums only)
-    kern<<<grid, 256, kActBwdMaxGroups * 512, s>>>(p);
+    kern<<<grid, 256, kActBwdMaxGroups * 512, s>>>(p);  // 16 KB: the rows' sums
     e = cudaGetLastError();
   } else {
     auto kern = gelu ? act_backward_kernel<kActGeluTanh, false> : act_backward_kernel<kActSilu, false>;
@@ -1721,9 +1720,10 @@ int ltxfp8_transpose_weight_128x128(const void* q, const float* sfb, int64_t N, 
 
 // ----------------------------------------------------------------------------- weight gradient
 // Kernel form, tile width and splits of the summed axis.  A cost model in clock cycles picks
-// among the one-CTA and the CTA-pair form, tile widths (multiples of 16, 64 to 256) and splits: a stage of 64 tokens costs what its form measured, a unit has a
-// fixed start and drain, the units run in waves over the SMs (or pairs of SMs), and split
-// partials are written and read back at L2 rates and cost one more launch.
+// among the one-CTA and the CTA-pair form, tile widths (multiples of 16, 64 to 256) and splits:
+// a stage of 64 tokens costs what its form measured, a unit has a fixed start and drain, the
+// units run in waves over the SMs (or pairs of SMs), and split partials are written and read
+// back at L2 rates and cost one more launch.
 // Cycles of a 64-token stage, fitted to one CTA at nt = 128 / 240 (1112 / 1340) and a pair at
 // nt = 128 / 192 / 256 (1040 / 1120 / 1300).
 static double wgrad_stage_cycles(bool pair, int nt) { return pair ? 760.0 + 2.1 * nt : 860.0 + 2.0 * nt; }

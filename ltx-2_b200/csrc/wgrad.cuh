@@ -5,9 +5,11 @@
 // g bf16 [M, N] is the gradient of the layer's output, x the layer's input as the forward
 // pass quantised it (e4m3 codes and 1x128 scales) or as bf16.  The scales vary along the
 // summed axis, so they cannot be applied to partial sums as the forward GEMM does; the
-// codes are expanded to bf16 on the way into the tensor core's operand tile instead (one
-// rounding per value, 2^-9 relative at most, which a sum over tokens averages out).  No
-// bf16 copy of x exists in memory.
+// codes are expanded to bf16 on the way into the tensor core's operand tile instead: one
+// rounding per value, 2^-8 of it at most and of either sign: about as much again as the result's
+// own rounding (0.0022 against 0.0017 in the root mean square, measured), and a 16th of the
+// codes' (e4m3, 2^-4).  Rounding the scales into g would round as often.  No bf16 copy of x
+// exists in memory.
 //
 // Both operands have the summed axis as their row axis, so they are MN-major operands of
 // tcgen05.mma.kind::f16, 64 tokens a stage.  A CTA computes a 256 (k) x nt (n <= 256) tile as
@@ -29,6 +31,10 @@
 // of operand reads (1500 cycles); in a pair the g tile is stored once per pair and each SM's
 // tensor core reads half of it: 144 KB (1150 cycles), and the traffic from L2 falls from 48 KB
 // to 32 KB a stage and SM.
+// Measured, 2 M N K / time: 6144 x 4096 x 4096 151 us (1366 TFLOP/s, tensor pipe 86 % active; the
+// library's product of bf16 operands, without the expansion, takes 138), 24576 x 4096 x 4096 565 us
+// (1460 TFLOP/s).  For few columns of g (LoRA factors) the expansion bounds it, 16 codes a cycle
+// and SM: 6143 x 32 x 4096 15 us and 24576 x 128 x 4096 38, against 4 and 17 of traffic.
 // The summed axis is divided among `splits` units where the tiles alone would not fill the
 // GPU; those write fp32 partials that wgrad_reduce_kernel adds in split order.
 #pragma once
