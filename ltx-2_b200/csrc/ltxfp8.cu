@@ -448,6 +448,21 @@ cudaError_t gated_launch(const DeviceInfo* d, cudaStream_t s, const __nv_bfloat1
     }                                                                                              \
   } while (0)
 
+// Bytes from the first to behind the last value of M bf16 rows.
+int64_t rows_bytes(int64_t ld, int64_t M, int64_t n) { return ((M - 1) * ld + n) * 2; }
+
+// Null pointers overlap nothing.
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
+
+// A contiguous bf16 [M, n] result and a row operand of the same shape: apart in memory, or the
+// same rows (each value is read before its place is written, but other rows' blocks run meanwhile).
+bool apart_or_in_place(const void* out, const void* in, int64_t in_ld, int64_t M, int64_t n) {
+  return (out == in && (in_ld == n || M == 1)) || !overlap(out, M * n * 2, in, rows_bytes(in_ld, M, n));
+}
+
 // Warps that share a row: one run of 16 values a thread up to H = 8192, two beyond.
 int norm_warps(int64_t H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
 int norm_block_rows(int64_t H) { return norm_warps(H) > 8 ? 1 : 8 / norm_warps(H); }
@@ -1295,14 +1310,14 @@ int ltxfp8_gemm_residual(const void* A, const float* sfa, int64_t sfa_ld, const 
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: unknown activation %d", activation);
   if (!A || !sfa || !W || !sfb || !D) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: null operand");
   if (sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: sfa_ld < M");
-  if (residual == D && residual_ld != N)
-    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: in place needs contiguous rows");
   if (residual && residual_ld < N) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: residual_ld < N");
   if (!aligned(A, 16) || !aligned(W, 16) || !aligned(D, 16) || (bias && !aligned(bias, 16)))
     return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: A, W, D and bias must be 16-byte aligned");
   if (!aligned(sfa, 4) || !aligned(sfb, 4)) return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: scales must be 4-byte aligned");
   if (residual && (!aligned(residual, 16) || residual_ld % 8 != 0))
     return fail(LTXFP8_ERR_MISALIGNED, "gemm_residual: residual must be 16-byte aligned with residual_ld %% 8 == 0");
+  if (!apart_or_in_place(D, residual, residual_ld, M, N))
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gemm_residual: D overlaps the residual; in place needs contiguous rows");
   DeviceInfo* d;
   int rc = device_info(&d);
   if (rc) return rc;
@@ -1381,8 +1396,8 @@ int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, 
   if (residual) {
     if ((rc = norm_rows(name, "residual", residual, residual_ld, H)) != 0) return rc;
     if ((rc = norm_rows(name, "h", h, H, H)) != 0) return rc;
-    if ((h == x && x_ld != H) || (h == residual && residual_ld != H))
-      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: in place needs contiguous rows", name);
+    if (!apart_or_in_place(h, x, x_ld, M, H) || !apart_or_in_place(h, residual, residual_ld, M, H))
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: h overlaps an input; in place needs contiguous rows", name);
   } else if (h) {
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: h is only written with a residual", name);
   }
@@ -1392,6 +1407,9 @@ int ltxfp8_rms_norm_quantize(const void* x, int64_t x_ld, const void* residual, 
     if (!aligned(q, 16) || !aligned(sfa, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: q must be 16-byte aligned", name);
   } else {
     if ((rc = norm_rows(name, "out", out, H, H)) != 0) return rc;
+    if (!apart_or_in_place(out, x, x_ld, M, H) || !apart_or_in_place(out, residual, residual_ld, M, H) ||
+        overlap(out, M * H * 2, h, M * H * 2))
+      return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: out overlaps an input or h; in place needs contiguous rows", name);
   }
   if (rstd && !aligned(rstd, 4)) return fail(LTXFP8_ERR_MISALIGNED, "%s: rstd must be 4-byte aligned", name);
   DeviceInfo* d;
@@ -1473,7 +1491,8 @@ int ltxfp8_rms_norm_backward(const void* dy, int64_t dy_ld, const void* h, int64
   if (dh && (rc = norm_rows(name, "dh", dh, dh_ld, H)) != 0) return rc;
   if ((rc = norm_rows(name, "dx", dx, H, H)) != 0) return rc;
   if (!rstd) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: rstd is null", name);
-  if (dx == h || (dx == dy && dy_ld != H) || (dx == dh && dh_ld != H))
+  if (overlap(dx, M * H * 2, h, rows_bytes(h_ld, M, H)) || !apart_or_in_place(dx, dy, dy_ld, M, H) ||
+      !apart_or_in_place(dx, dh, dh_ld, M, H))
     return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: dx may only be dy or dh, with contiguous rows", name);
   if (!aligned(rstd, 4) || (dweight && !aligned(dweight, 4)))
     return fail(LTXFP8_ERR_MISALIGNED, "%s: rstd and dweight must be 4-byte aligned", name);
@@ -1645,7 +1664,8 @@ int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const flo
   if ((rc = act_codes(name, "z", zq, zs, zs_ld, M)) != 0) return rc;
   if (!dz && !dzq) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: need dz or dzq", name);
   if (dz && (rc = norm_rows(name, "dz", dz, N, N)) != 0) return rc;
-  if (dz == dy && dy_ld != N) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: in place needs contiguous rows", name);
+  if (!apart_or_in_place(dz, dy, dy_ld, M, N))
+    return fail(LTXFP8_ERR_INVALID_ARGUMENT, "%s: dz overlaps dy; in place needs contiguous rows", name);
   if (dzq && (rc = act_codes(name, "dz", dzq, dzs, dzs_ld, M)) != 0) return rc;
   DeviceInfo* d;
   rc = device_info(&d);

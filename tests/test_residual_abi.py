@@ -132,6 +132,15 @@ def test_in_place_needs_contiguous_rows():
         assert lib.ltxfp8_rms_norm_backward(P, dy_ld, h, 256, P, None, 0, 3 * P, dh_ld, 4, 256, dx, None, None, 0,
                                             None) == A
     assert lib.ltxfp8_gemm_residual(P, P, 8, P, P, None, Q, 512, Q, 8, 256, 256, 0, None, 0, None) == A
+    # results shifted against an operand by some rows
+    assert lib.ltxfp8_gemm_residual(P, P, 8, P, P, None, Q, 256, Q + 512, 8, 256, 256, 0, None, 0, None) == A
+    assert lib.ltxfp8_rms_norm_quantize(P, 256, Q, 256, 4, 256, None, 0, 1e-6, P + 512, 3 * P, P, 4, None, None, None) == A
+    assert lib.ltxfp8_rms_norm_quantize(P, 256, None, 0, 4, 256, None, 0, 1e-6, None, None, None, 4, P + 1024, None,
+                                        None) == A
+    assert lib.ltxfp8_rms_norm_quantize(P, 256, Q, 256, 4, 256, None, 0, 1e-6, 3 * P, None, None, 4, 3 * P, None,
+                                        None) == A  # out is h
+    assert lib.ltxfp8_rms_norm_backward(P, 256, Q, 256, P, None, 0, None, 0, 4, 256, Q + 512, None, None, 0, None) == A
+    assert lib.ltxfp8_act_backward(P, 256, Q, P, 4, 4, 256, 1, P + 512, None, None, 4, None, None, 0, None) == A
     assert lib.ltxfp8_act_backward(P, 512, Q, P, 4, 4, 256, 1, P, None, None, 4, None, None, 0, None) == A
 
 
