@@ -112,16 +112,17 @@ struct ActBwdParams {
 // about 20 others a value) hides the loads only if many are in flight, so bulk copies bring
 // dy and the codes through a ring of shared-memory stages.  A stage is released by one
 // arrival per warp as soon as its values are in registers.
-// Measured with dz in both forms and dbias at 6143 x 16384: 111 us, 5.5 TB/s (floor 94 us of
-// traffic); loads to registers alone took 134 us where the first ring took 122.
+// Measured with dz in both forms and dbias at 6143 x 16384: 107 us, 5.7 TB/s (floor 94 us of
+// traffic); three stages (108 KB in flight on an SM) are best: two 109, four 109, six 111; loads to
+// registers alone took 134 us where the first ring took 122.
 // kDirect: a few rows (one share, so no partial sums and no second launch): the loads go straight
 // to registers.
 enum ActStatus : unsigned int { kStActLoad = 0x41010001u, kStActFree = 0x41010002u, kStActDrain = 0x41010003u };
 constexpr int kActBwdMaxGroups = 32;  // 4096 columns = 256 threads x 16
-constexpr int kActBwdStages = 6;
+constexpr int kActBwdStages = 3;
 constexpr uint32_t kActBwdDyBytes = kActBwdMaxGroups * 256;                    // 8 KB a pass
 constexpr uint32_t kActBwdStageBytes = kActBwdDyBytes + kActBwdMaxGroups * 128;  // + 4 KB of codes
-constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 72 KB: three blocks an SM
+constexpr uint32_t kActBwdSmemBytes = kActBwdStages * kActBwdStageBytes;       // 36 KB
 
 template <int kAct, bool kDirect>
 __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams p) {
