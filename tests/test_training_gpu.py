@@ -373,6 +373,45 @@ def test_operators_on_another_stream(cuda_device):
         assert torch.equal(a, b)
 
 
+def test_two_threads_on_two_streams(cuda_device):
+    """Calls from two host threads at once, each on its own stream: nothing is shared between them."""
+    import threading
+
+    from ltx_kernels.blockwise import ops
+    w, s = _weight(384, 640, cuda_device, 131)
+    ins = [(tokens(m, 640, 132 + m).to(cuda_device), grads(m, 384, 133 + m).to(cuda_device)) for m in (12, 700)]
+
+    def chain(x, g):
+        q, sc, h, rstd = ops.rms_norm_quantize(x, None, x)
+        z = ops.gemm_residual(q, sc, w, s, residual=g, activation="silu")
+        yq, ys, zq, zs = ops.act_quantize_save(z)
+        dz, dq, ds, db = ops.act_backward(g, zq, zs, quantize=True, dbias=True)
+        dx, dw = ops.rms_norm_backward(x, h, rstd, torch.ones(640, device=cuda_device), h)
+        return [z, yq.float(), dz, ds, db, dx, dw, ops.wgrad_1x128(dz, q, sc)]
+
+    want = [chain(*i) for i in ins]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()) as _:
+                for _ in range(20):
+                    got = chain(*ins[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_operators_in_cuda_graphs(cuda_device):
     """Captured once and replayed on new inputs, two graphs in turn: each has workspaces of its own."""
     from ltx_kernels.blockwise import ops
