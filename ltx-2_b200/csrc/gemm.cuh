@@ -127,8 +127,6 @@ struct GemmParams {
   int k_splits;
   int kb_per_split;
   float* ws;
-  const __nv_bfloat16* res;  // residual [M, N], row stride res_ld (kGemmResidual)
-  int64_t res_ld;
 };
 
 // Grouped rasterisation: consecutive tile indices walk group_m M-tiles down a
@@ -280,7 +278,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     mbar_init(stg_full, 8);      // one arrival per promotion warp
     mbar_init(stg_empty, 2);     // one arrival per store warp
     mbar_init(drain, 1);
-    mbar_init(res_full, 2);      // one arrival per store warp
+    if constexpr (kAct >= 0) mbar_init(res_full, 2);  // one arrival per store warp
     fence_mbarrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -307,9 +305,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp < 4) {
     setmaxnreg_dec<kRegsCtrl>();
-    // The producer's and the issuer's loops run warp-uniform, one elected lane issuing (2-3 %
-    // faster than one thread of each warp: 6144 x 4096 x 4096 103 -> 100 us).
-    if (warp == 0) {
+    // The producer's and the issuer's loops run warp-uniform, one elected lane issuing (1-4 %
+    // faster than one thread of each warp: 6144 x 4096 x 4096 109 -> 107 us, with GELU and
+    // requantisation 156 -> 151), but for GELU without requantisation (131 -> 133).
+    constexpr bool kWarpLoops = !kGelu || kRequant;
+    auto wait = [](uint64_t* bar, uint32_t parity, unsigned int code) {
+      if constexpr (kWarpLoops) return warp_wait(bar, parity, code);
+      else return mbar_wait(bar, parity, code);
+    };
+    auto issuing = [] {
+      if constexpr (kWarpLoops) return elect_one();
+      else return true;
+    };
+    auto join = [] {
+      if constexpr (kWarpLoops) __syncwarp();
+    };
+    const bool in_loops = kWarpLoops || lane == 0;
+    if (warp == 0 && in_loops) {
       // ------------------------------------------------------------ TMA producer
       uint32_t it = 0;
       bool ok = true;
@@ -320,13 +332,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int m0 = w.mt * kBM, n0 = w.nt * kBN;
         for (int kb = 0; kb < w.n_blocks; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
-          if (!warp_wait(&empty[s], ph ^ 1u, kStProducerEmpty)) {
+          if (!wait(&empty[s], ph ^ 1u, kStProducerEmpty)) {
             ok = false;
             break;
           }
           uint8_t* sa = smem + s * kStageBytes;
           uint8_t* sb = sa + kABytes;
-          if (elect_one()) {
+          if (issuing()) {
             mbar_arrive_expect_tx(&full[s], kb < w.n_fp8 ? tx_fp8 : kStageBytes);
             if (kb < w.n_fp8) {
               tma_load_2d(&tmA, &full[s], sa, (w.kb_begin + kb) * kBK, m0);
@@ -337,15 +349,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               tma_load_2d(&tmLB, &full[s], sb, c, n0);
             }
           }
-          __syncwarp();
+          join();
         }
       }
       if (!ok) {
         // Let the loads already in flight land before the CTA exits.
         const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
-        for (uint32_t i = first; i < it; ++i) warp_wait(&full[i % kStages], (i / kStages) & 1u, kStDrain);
+        for (uint32_t i = first; i < it; ++i) wait(&full[i % kStages], (i / kStages) & 1u, kStDrain);
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && in_loops) {
       // ------------------------------------------------------------ MMA issuer
       constexpr uint32_t kIdescF8 = make_idesc(0u, kBM, kBN);
       constexpr uint32_t kIdescBF16 = make_idesc(1u, kBM, kBN);
@@ -358,12 +370,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int kb = 0; kb < w.n_blocks; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
           const uint32_t buf = it & 1u, bph = (it >> 1) & 1u;
-          if (!warp_wait(&tempty[buf], bph ^ 1u, kStMmaTmemEmpty)) {
+          if (!wait(&tempty[buf], bph ^ 1u, kStMmaTmemEmpty)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          if (!warp_wait(&full[s], ph, kStMmaFull)) {
+          if (!wait(&full[s], ph, kStMmaFull)) {
             ok = false;
             break;
           }
@@ -372,7 +384,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint64_t adesc = sw128_kmajor_desc(a_addr);
           const uint64_t bdesc = sw128_kmajor_desc(a_addr + kABytes);
           const uint32_t d_tmem = tmem_base + buf * kBN;
-          if (elect_one()) {
+          if (issuing()) {
             if (kb < w.n_fp8) {
 #pragma unroll
               for (int j = 0; j < 4; ++j)  // 4 x K32 (32 B of each 128 B row)
@@ -385,13 +397,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tc_commit(&empty[s]);
             tc_commit(&tfull[buf]);
           }
-          __syncwarp();
+          join();
         }
       }
       // Every MMA issued above has completed once `drain` flips.
-      if (elect_one()) tc_commit(drain);
-      __syncwarp();
-      warp_wait(drain, 0u, kStDrain);
+      if (issuing()) tc_commit(drain);
+      join();
+      wait(drain, 0u, kStDrain);
     } else if (warp >= 2 && p.k_splits == 1) {
       // ------------------------------------------------------------ staging -> global (warps 2, 3)
       // Warp pw owns the 32-row slices pw*32 and 64 + pw*32 of the tile: its passes and stores need
@@ -671,7 +683,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // row, 128-column group): 16 lanes x 8 columns, so the 1x128 requantisation needs
 // no cross-row reduction.  Epilogue semantics are those of the GEMM kernel.
 template <bool kGelu, bool kRequant, int kAct = -1>
-__global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmParams p) {
+__global__ void __launch_bounds__(256)
+    splitk_reduce_kernel(const GemmParams p, const __nv_bfloat16* __restrict__ res, int64_t res_ld) {
   const int64_t total = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int l16 = threadIdx.x & 15;
@@ -716,7 +729,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const GemmParams p) 
   if constexpr (kAct >= 0) {
     uint4 rv = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
     if (active && (p.flags & kGemmResidual))
-      rv = *reinterpret_cast<const uint4*>(p.res + static_cast<int64_t>(row) * p.res_ld + col);
+      rv = *reinterpret_cast<const uint4*>(res + static_cast<int64_t>(row) * res_ld + col);
     const float2 z = make_float2(0.0f, 0.0f);  // the bias is in f already
     if (active)
       *reinterpret_cast<uint4*>(p.d + off) = make_uint4(residual_pair<kAct>(make_float2(f[0], f[1]), z, rv.x),

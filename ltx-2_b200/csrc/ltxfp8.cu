@@ -276,14 +276,15 @@ int gemm_plan_launches(const GemmPlan& g) {
 }
 
 template <bool kGelu, bool kRequant, int kAct = -1>
-int splitk_reduce_launch(const DeviceInfo* d, const GemmParams& p, cudaStream_t stream) {
+int splitk_reduce_launch(const DeviceInfo* d, const GemmParams& p, const __nv_bfloat16* res, int64_t res_ld,
+                         cudaStream_t stream) {
   const int64_t groups = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const unsigned blocks = static_cast<unsigned>((groups + 15) / 16);
   cudaError_t e;
   if constexpr (kAct >= 0) {
-    e = launch_dependent(splitk_reduce_kernel<kGelu, kRequant, kAct>, blocks, 256, stream, p);
+    e = launch_dependent(splitk_reduce_kernel<kGelu, kRequant, kAct>, blocks, 256, stream, p, res, res_ld);
   } else {
-    splitk_reduce_kernel<kGelu, kRequant, kAct><<<blocks, 256, 0, stream>>>(p);
+    splitk_reduce_kernel<kGelu, kRequant, kAct><<<blocks, 256, 0, stream>>>(p, nullptr, 0);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return cuda_fail(e, "split-K reduce launch");
@@ -294,10 +295,10 @@ int splitk_reduce_launch(const DeviceInfo* d, const GemmParams& p, cudaStream_t 
 template <bool kGelu, bool kRequant, int kAct = -1>
 int gemm_launch_full(DeviceInfo* d, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& lx,
                      const CUtensorMap& lb, const CUtensorMap& md, const CUtensorMap& mq, const GemmParams& p,
-                     cudaStream_t stream) {
+                     cudaStream_t stream, const __nv_bfloat16* res = nullptr, int64_t res_ld = 0) {
   int rc = gemm_launch<kGelu, kRequant, kAct>(d, a, b, lx, lb, md, mq, p, stream);
   if (rc || p.k_splits == 1) return rc;
-  return splitk_reduce_launch<kGelu, kRequant, kAct>(d, p, stream);
+  return splitk_reduce_launch<kGelu, kRequant, kAct>(d, p, res, res_ld, stream);
 }
 
 template <bool kGelu, bool kRequant>
@@ -1060,19 +1061,19 @@ static int gemm_rows(DeviceInfo* d, const void* A, const float* sfa, int64_t sfa
     }
   }
   if (re) {
-    if (re->res) {
-      p.res = re->res + row0 * re->res_ld;
-      p.res_ld = re->res_ld;
+    const __nv_bfloat16* res = re->res ? re->res + row0 * re->res_ld : nullptr;
+    if (res) {
       p.flags |= kGemmResidual;
       if (!split) {
-        rc = make_map_2d(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.res, N, rows, re->res_ld * 2, 64, 32);
+        rc = make_map_2d(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, res, N, rows, re->res_ld * 2, 64, 32);
         if (rc) return rc;
       }
     }
     if (re->act == kActGeluTanh)
-      return gemm_launch_full<false, false, kActGeluTanh>(d, ma, mb, mlx, mlb, md, mq, p, stream);
-    if (re->act == kActSilu) return gemm_launch_full<false, false, kActSilu>(d, ma, mb, mlx, mlb, md, mq, p, stream);
-    return gemm_launch_full<false, false, kActNone>(d, ma, mb, mlx, mlb, md, mq, p, stream);
+      return gemm_launch_full<false, false, kActGeluTanh>(d, ma, mb, mlx, mlb, md, mq, p, stream, res, re->res_ld);
+    if (re->act == kActSilu)
+      return gemm_launch_full<false, false, kActSilu>(d, ma, mb, mlx, mlb, md, mq, p, stream, res, re->res_ld);
+    return gemm_launch_full<false, false, kActNone>(d, ma, mb, mlx, mlb, md, mq, p, stream, res, re->res_ld);
   }
   if (use_pair) {
     if (gelu && requant) return gemm_pair_launch<true, true>(d, ma, mb, mlx, mlb, md, mq, p, stream);
