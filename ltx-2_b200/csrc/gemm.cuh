@@ -104,6 +104,8 @@ enum GemmStatus : unsigned int {
   kStResidual = 0x47010008u,
 };
 
+// (Two more words in here, the residual's, cost every instantiation 16 to 32 bytes of spills in its
+// promotion loop: the split-K reduction, which alone reads them, gets them beside it.)
 struct GemmParams {
   int M, N, K;
   int num_kb;         // K / 128
