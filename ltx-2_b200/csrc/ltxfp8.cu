@@ -1747,6 +1747,9 @@ int ltxfp8_transpose_weight_128x128(const void* q, const float* sfb, int64_t N, 
 // back at L2 rates and cost one more launch.
 // Cycles of a 64-token stage, fitted to one CTA at nt = 128 / 240 (1112 / 1340) and a pair at
 // nt = 128 / 192 / 256 (1040 / 1120 / 1300).
+// A launch of pairs starts later (0.4 to 1 us: 6143 x 32 x 4096 14.9 us with single CTAs, 15.3 in
+// pairs; 716 x 64 x 3328 8.4 / 9.7; 300 x 1024 x 1024 8.0 / 9.0), which only long units make up for.
+constexpr double kWgPairStart = 1500.0;
 static double wgrad_stage_cycles(bool pair, int nt) { return pair ? 760.0 + 2.1 * nt : 860.0 + 2.0 * nt; }
 
 struct WgradPlan {
@@ -1784,7 +1787,8 @@ static WgradPlan wgrad_plan(int sms, int64_t M, int64_t N, int64_t K) {
         const double unit = static_cast<double>(per) * stage + 3000.0 + 16.0 * nt;
         const int64_t waves = (tiles * s + slots - 1) / slots;
         const double ws = s > 1 ? static_cast<double>(tiles * s) * (1 + pair) * nt * kWgTileK * 4.0 : 0.0;
-        const double cost = static_cast<double>(waves) * unit + (s > 1 ? 4000.0 + ws / 1500.0 : 0.0);
+        const double cost = static_cast<double>(waves) * unit + (s > 1 ? 4000.0 + ws / 1500.0 : 0.0) +
+                            (pair ? kWgPairStart : 0.0);
         if (ws <= 512.0 * 1048576.0 && tiles * s <= 0x3FFFFFFF && (best.nt == 0 || cost < best_cost)) {
           best_cost = cost;
           best = WgradPlan{pair != 0,

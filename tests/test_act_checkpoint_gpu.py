@@ -164,7 +164,7 @@ def test_wgrad_forms(cuda_device):
     seen = set()
     sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
     for M, N, K in ((333, 48, 384), (5001, 144, 1152), (77, 2064, 1152), (333, 2064, 384), (1001, 528, 2176),
-                    (2001, 144, 896), (5001, 2064, 896)):
+                    (2001, 144, 896), (5001, 2064, 896), (2068, 832, 2176), (4175, 1536, 1920), (24577, 128, 640)):
         i = _lib.WgradPlanInfo()
         assert _lib.load().ltxfp8_wgrad_plan_for_sms(M, N, K, sms, ctypes.byref(i)) == _lib.OK
         seen.add((bool(i.pair), i.splits > 1))
