@@ -405,7 +405,7 @@ int ltxfp8_act_quantize_save(const void* z, int64_t z_ld, int64_t M, int64_t N, 
 /*
  * Its gradient from the checkpoint: dz = dy * act'(zq * zs), written as bf16 (dz), as
  * 1x128 codes (dzq, dzs) or both, and dbias fp32 [N] = sum over rows of dz (NULL: not
- * wanted; it needs a workspace of ltxfp8_act_backward_workspace_bytes).  dz may be dy when
+ * wanted; it needs a workspace of ltxfp8_act_backward_workspace_bytes, 0: none).  dz may be dy when
  * that is contiguous.  M == 0 gives dbias = 0.
  */
 int ltxfp8_act_backward(const void* dy, int64_t dy_ld, const void* zq, const float* zs, int64_t zs_ld, int64_t M,

@@ -8,9 +8,10 @@
 // CTAs, a workspace of partial sums and a second launch; here a block owns 16 weight rows, each
 // of its 8 warps an eighth of their K blocks (consecutive, so that a row is read in long
 // stretches), and mma.sync m16n8k32 multiplies 16 weight rows by 8 tokens straight from registers:
-// nothing passes through shared memory but the eight warps' sums at the end.  Within a K block the products may be summed in any order, so a lane
-// takes the 32 bytes of a row that two 16-byte loads give it (bytes 16 t and 64 + 16 t, t = lane
-// % 4) as its fragments, the same bytes of the weight and of the tokens.
+// nothing passes through shared memory but the eight warps' sums at the end.  Within a K block the
+// products may be summed in any order, so a lane takes the 32 bytes of a row that two 16-byte
+// loads give it (bytes 16 t and 64 + 16 t, t = lane % 4) as its fragments, the same bytes of the
+// weight and of the tokens.
 #pragma once
 
 #include "gemm.cuh"
