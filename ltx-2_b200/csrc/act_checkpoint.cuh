@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256, 3) act_backward_kernel(const ActBwdParams
     const int s = j % kActBwdStages;
     const uint32_t ph = (j / kActBwdStages) & 1u;
     const bool in = mine && m < p.M;
-    const float sc = sc_next;
+    const float sc = act_grad_scale(sc_next);
     sc_next = (mine && m + step < p.M) ? __ldg(zs + m + step) : 0.0f;
     Run16 vy = zero_run();
     uint4 vz = make_uint4(0, 0, 0, 0);

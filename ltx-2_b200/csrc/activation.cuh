@@ -40,6 +40,10 @@ __device__ __forceinline__ float2 act_apply(const float2 z) {
 
 // With q = z u'(z): act' = s + s (q - q s).  q - q s is one fused step, so 1 - s loses nothing
 // where s is small; where s is near 1 the term is an absolute error of 2^-24 q in a value near 1.
+// GELU's q is a cubic: |z| has to stay below 10^12 (act_grad_scale), or an infinite q meets 1 - s = 0
+// or s = 0.  Where e vanishes, s has to be 1 exactly: the approximate reciprocal of 1.0 is 1.0, which
+// test_act_extremes_gpu.py holds to (an ulp less would be 2^-24 q).  Forming q from at most z = 16, which
+// would not need that, costs an instruction a value: 6143 x 16384 106.5 -> 110.5 us.
 template <int kAct>
 __device__ __forceinline__ float2 act_grad(const float2 z) {
   const float2 d = __fadd2_rn(act_exp<kAct>(z), make_float2(1.0f, 1.0f));
@@ -53,5 +57,10 @@ __device__ __forceinline__ float2 act_grad(const float2 z) {
   const float2 v = __ffma2_rn(make_float2(-s.x, -s.y), q, q);
   return __ffma2_rn(s, v, s);
 }
+
+// The scale of a group of e4m3 codes that act_grad is taken of, at most 2^16 (|z| < 2^25): the
+// smallest code but zero, 2^-9, is 128 there, where the derivative of either activation has become 0
+// or 1 to fp32, so a larger scale changes nothing.  Infinity and NaN stay.
+__device__ __forceinline__ float act_grad_scale(float s) { return isfinite(s) ? fminf(s, 65536.0f) : s; }
 
 }  // namespace ltxfp8
