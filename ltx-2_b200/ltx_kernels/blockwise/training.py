@@ -105,7 +105,6 @@ class _LinearTrain(torch.autograd.Function):
         ctx.x_meta = (x.shape, x.dtype)
         ctx.master_dtype = None if master is None else master.dtype
         ctx.lora_dtypes = (None, None) if lora_a is None else (lora_a.dtype, lora_b.dtype)
-        ctx.residual_shape = None if residual is None else residual.shape
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
@@ -133,7 +132,9 @@ class _LinearTrain(torch.autograd.Function):
         if need_b:
             db = ops.wgrad_bf16(ax, g, alpha=ctx.alpha, transposed=True).to(ctx.lora_dtypes[1])
         if need_r:
-            dr = g.view(ctx.residual_shape)
+            # The tensor itself: a view of it would be a new object over the same memory, which autograd
+            # takes over as a leaf's .grad although the caller, or another leaf, still holds dy.
+            dr = dy
         return dx, dw, dbias, da, db, dr, None, None, None, None
 
 

@@ -1,0 +1,75 @@
+"""How the training functions stand in an autograd graph: gradients with storage of their own,
+outputs that can be modified in place, layers above and below, captures."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from residual_inputs import act64, dequant_weight64, gen, grads, quant_weight, tokens
+
+pytestmark = pytest.mark.gpu
+
+# e4m3's rounding in the root mean square, at worst uniformly spread over half a step
+E4M3_RMS = 2.0 ** -4 / 3 ** 0.5
+
+
+def _rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return ((a - b).norm() / b.norm()).item()
+
+
+def _weight(N, K, dev, seed):
+    q, s = quant_weight(torch.randn(N, K, generator=gen(seed)) / K ** 0.5)
+    return q.to(dev), s.to(dev)
+
+
+def _leaf(t, dev):
+    return t.to(dev).requires_grad_()
+
+
+def _bf16(*shape, seed, scale=1.0):
+    return (scale * torch.randn(*shape, generator=gen(seed))).to(torch.bfloat16)
+
+
+# ----------------------------------------------------------------------------- storage
+@pytest.mark.parametrize("lead", [(24,), (2, 12)])
+@pytest.mark.parametrize("lora", [False, True])
+def test_residual_gradients_have_their_own_storage(cuda_device, lead, lora):
+    """Two linears, each with a residual of its own, summed; three steps accumulate into the
+    leaves: each gradient is three times one step's, and the caller's gradient is untouched."""
+    from ltx_kernels.blockwise import fp8_linear_train
+    K, N = 128, 256
+    w = _weight(N, K, cuda_device, 1)
+    ab = (_bf16(16, K, seed=2).to(cuda_device), _bf16(N, 16, seed=3).to(cuda_device), 0.5) if lora else None
+    x = tokens(24, K, 4).view(*lead, K).to(cuda_device)
+    r1, r2 = (_leaf(tokens(24, N, s).view(*lead, N), cuda_device) for s in (5, 6))
+    dy = (grads(24, N, 7).view(*lead, N) * 1e3).to(cuda_device)
+    kept = dy.clone()
+    for _ in range(3):
+        y = fp8_linear_train(x, w, lora=ab, residual=r1) + fp8_linear_train(x, w, lora=ab, residual=r2)
+        y.backward(dy)
+    assert torch.equal(dy, kept)
+    want = kept + kept + kept  # bf16, as the accumulation rounds
+    assert torch.equal(r1.grad, want) and torch.equal(r2.grad, want)
+    assert r1.grad.data_ptr() != r2.grad.data_ptr()
+    # the output's gradient handed in directly
+    r1.grad = r2.grad = None
+    for _ in range(2):
+        fp8_linear_train(x, w, lora=ab, residual=r1).backward(dy)
+    assert torch.equal(dy, kept) and torch.equal(r1.grad, kept + kept) and r1.grad.data_ptr() != dy.data_ptr()
+
+
+def test_block_gradients_have_their_own_storage(cuda_device):
+    """x and the residual of a block share the values of their gradient, not its memory."""
+    from ltx_kernels.blockwise import pre_norm_feed_forward
+    d, inner = 128, 256
+    w1, w2 = _weight(inner, d, cuda_device, 11), _weight(d, inner, cuda_device, 12)
+    x, r = (_leaf(tokens(24, d, s).view(2, 12, d), cuda_device) for s in (13, 14))
+    dy = (grads(24, d, 15).view(2, 12, d) * 1e3).to(cuda_device)
+    kept = dy.clone()
+    grad = torch.autograd.grad(pre_norm_feed_forward(x, w1, w2, residual=r), x, dy)[0]
+    for _ in range(3):
+        pre_norm_feed_forward(x, w1, w2, residual=r).backward(dy)
+    assert torch.equal(dy, kept) and x.grad.data_ptr() != r.grad.data_ptr()
+    want = grad + grad + grad
+    assert torch.equal(x.grad, want) and torch.equal(r.grad, want)
