@@ -55,6 +55,13 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t
 
 
+def _empty_output(x: torch.Tensor, N: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A bf16 result [..., N] for x [..., K], and its rows [M, N].  The operators write the rows and the
+    Function returns the result: a view of what they return could not be modified in place."""
+    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+    return out, out.view(-1, N)
+
+
 def _check_capture(name: str, *leaves: Optional[torch.Tensor]) -> None:
     """Refuse, while a CUDA graph is captured, leaves whose gradient node was made on the default
     stream and is still alive (an earlier eager result that has not been released): autograd
@@ -87,15 +94,16 @@ class _LinearTrain(torch.autograd.Function):
         x2 = _rows(x, K)
         q, s = ops.quantize_1x128(x2, quant_mode)
         ax = a = b = None
+        y, rows = _empty_output(x, N)
         if lora_a is not None:
             a, b = lora_a.to(torch.bfloat16), lora_b.to(torch.bfloat16)
             ax = ops.lora_a(x2, a)
-            y = ops.gemm(q, s, w_q, w_s, bias, lora_ax=ax, lora_b=b, lora_alpha=alpha)
+            ops.gemm(q, s, w_q, w_s, bias, out=rows, lora_ax=ax, lora_b=b, lora_alpha=alpha)
             if residual is not None:
-                y = y + residual.reshape(-1, N)
+                y += residual
         else:
-            y = ops.gemm_residual(q, s, w_q, w_s, bias,
-                                  residual=None if residual is None else residual.reshape(-1, N))
+            ops.gemm_residual(q, s, w_q, w_s, bias, out=rows,
+                              residual=None if residual is None else residual.reshape(-1, N))
         # Only what the wanted gradients read: the codes for the weight or A, x A^T for B.
         need_x, need_w, _, need_a, need_b = ctx.needs_input_grad[:5]
         if not (need_w or need_a):
@@ -105,7 +113,7 @@ class _LinearTrain(torch.autograd.Function):
         ctx.x_meta = (x.shape, x.dtype)
         ctx.master_dtype = None if master is None else master.dtype
         ctx.lora_dtypes = (None, None) if lora_a is None else (lora_a.dtype, lora_b.dtype)
-        return y.view(*x.shape[:-1], N)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -202,7 +210,8 @@ class _PreNormFeedForward(torch.autograd.Function):
         need_x, need_r, need_nw, need_w1, need_b1, need_w2, _ = ctx.needs_input_grad[:7] if train else (False,) * 7
         below = need_x or need_r or need_nw
         yq, ys, zq, zs = ops.act_quantize_save(z, activation, save=below or need_w1 or need_b1)
-        out = ops.gemm_residual(yq, ys, w2, s2, b2, residual=h)
+        out, rows = _empty_output(x, K)
+        ops.gemm_residual(yq, ys, w2, s2, b2, residual=h, out=rows)
         if train:
             keep = lambda want, *ts: ts if want else (None,) * len(ts)  # noqa: E731
             ctx.save_for_backward(*keep(need_w1, nq, ns), *keep(below, h, rstd), zq, zs, *keep(need_w2, yq, ys),
@@ -210,7 +219,7 @@ class _PreNormFeedForward(torch.autograd.Function):
         ctx.activation = activation
         ctx.shape = x.shape
         ctx.master_dtypes = tuple(None if m is None else m.dtype for m in (m1, m2))
-        return out.view(x.shape)
+        return out
 
     @staticmethod
     @once_differentiable

@@ -73,3 +73,28 @@ def test_block_gradients_have_their_own_storage(cuda_device):
     assert torch.equal(dy, kept) and x.grad.data_ptr() != r.grad.data_ptr()
     want = grad + grad + grad
     assert torch.equal(x.grad, want) and torch.equal(r.grad, want)
+
+
+# ----------------------------------------------------------------------------- in place
+@pytest.mark.parametrize("lead", [(24,), (2, 12)])
+@pytest.mark.parametrize("which", ["linear", "lora", "block"])
+def test_outputs_can_be_modified_in_place(cuda_device, lead, which):
+    """``y += skip`` and an in-place activation on the output: the same gradients as out of place."""
+    from ltx_kernels.blockwise import fp8_linear_train, pre_norm_feed_forward
+    K = 128
+    w1, w2 = _weight(256, K, cuda_device, 21), _weight(K, 256, cuda_device, 22)
+    a, b = _leaf(_bf16(16, K, seed=23), cuda_device), _leaf(_bf16(256, 16, seed=24), cuda_device)
+    x = _leaf(tokens(24, K, 25).view(*lead, K), cuda_device)
+    call = {"linear": lambda: fp8_linear_train(x, w1), "lora": lambda: fp8_linear_train(x, w1, lora=(a, b, 0.5)),
+            "block": lambda: pre_norm_feed_forward(x, w1, w2)}[which]
+    skip = _leaf(tokens(24, call().shape[-1], 26).view(*lead, -1), cuda_device)
+    dy = (grads(24, skip.shape[-1], 27).view(*lead, -1) * 1e3).to(cuda_device)
+    y = call()
+    y += skip
+    y.relu_()
+    got = torch.autograd.grad(y, (x, skip), dy)
+    z = torch.relu(call() + skip)
+    want = torch.autograd.grad(z, (x, skip), dy)
+    assert torch.equal(y, z) and y.shape == (*lead, skip.shape[-1])
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
