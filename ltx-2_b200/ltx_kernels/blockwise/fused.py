@@ -24,7 +24,7 @@ import torch.nn as nn
 from .. import _lib as L
 from . import ops
 from .functional import blockwise_quantize_triton, quant_mode_code
-from .linear import BlockwiseFP8Linear
+from .linear import BlockwiseFP8Linear, wants_gradient
 
 Activation = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
 
@@ -124,8 +124,7 @@ class BlockwiseFP8LoRALinear(BlockwiseFP8Linear):
     def forward(self, x):
         if isinstance(x, tuple):
             raise RuntimeError("BlockwiseFP8LoRALinear needs the bf16 input for the LoRA term")
-        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad
-                                        or (self.bias is not None and self.bias.requires_grad)):
+        if wants_gradient(x, self.lora_A, self.lora_B, self.bias):
             from .training import fp8_linear_train
             return fp8_linear_train(x, (self.weight, self.weight_scale), self.bias,
                                     lora=(self.lora_A, self.lora_B, self.alpha),

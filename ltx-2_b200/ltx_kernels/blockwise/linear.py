@@ -70,6 +70,13 @@ def is_16bit(x) -> bool:
     return x.dtype == torch.float16 or x.dtype == torch.bfloat16
 
 
+def wants_gradient(x, *params: Optional[torch.Tensor]) -> bool:
+    """Whether a layer's call has to be differentiable: gradients are enabled and its input (not a
+    quantised pair, which cannot carry one) or one of its parameters requires one."""
+    return torch.is_grad_enabled() and isinstance(x, torch.Tensor) and (
+        x.requires_grad or any(p is not None and p.requires_grad for p in params))
+
+
 class BlockwiseGemmLinearFunc(torch.autograd.Function):
     """Forward-only blockwise FP8 linear (linear.py:82-104): quantise a bf16 input
     (or take a pre-quantised ``(e4m3, scales)`` pair), GEMM, view to ``(b, n, out)``."""
@@ -119,7 +126,12 @@ class BlockwiseLinear(nn.Module):
 
 class BlockwiseFP8Linear(BlockwiseLinear):
     """e4m3 weight ``[out, in]`` with fp32 128x128 block scales ``[out/128, in/128]``
-    (linear.py:151-209)."""
+    (linear.py:151-209).
+
+    The weight is frozen.  Where gradients are enabled and the input or the bias requires one, the
+    forward is differentiable (:func:`training.frozen_linear`), so that trainable layers below it
+    get theirs: the same output, but an all-zero 1x128 group of the input, NaN otherwise, counts as
+    zeros.  (The reference's is forward-only and its output detached.)"""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -134,6 +146,12 @@ class BlockwiseFP8Linear(BlockwiseLinear):
     @property
     def fp8weight(self):
         return self.weight
+
+    def forward(self, x):
+        if wants_gradient(x, self.bias):
+            from .training import frozen_linear
+            return frozen_linear(x, self.weight, self.weight_scale, self.bias)
+        return super().forward(x)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, transform_weights=True):

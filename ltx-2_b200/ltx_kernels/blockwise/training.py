@@ -26,6 +26,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
 from . import ops
+from .functional import quant_mode_code
 from .linear import BlockwiseFP8Linear
 
 Weight = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
@@ -88,7 +89,7 @@ def _bf16_grad(g: torch.Tensor, width: int) -> torch.Tensor:
 
 class _LinearTrain(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, master, bias, lora_a, lora_b, residual, w_q, w_s, alpha, quant_mode):
+    def forward(ctx, x, master, bias, lora_a, lora_b, residual, w_q, w_s, alpha, quant_mode, plain):
         _check_capture("fp8_linear_train", x, master, bias, lora_a, lora_b, residual)
         K, N = x.shape[-1], w_q.shape[0]
         x2 = _rows(x, K)
@@ -101,6 +102,8 @@ class _LinearTrain(torch.autograd.Function):
             ops.gemm(q, s, w_q, w_s, bias, out=rows, lora_ax=ax, lora_b=b, lora_alpha=alpha)
             if residual is not None:
                 y += residual
+        elif plain:
+            ops.gemm(q, s, w_q, w_s, bias, out=rows)
         else:
             ops.gemm_residual(q, s, w_q, w_s, bias, out=rows,
                               residual=None if residual is None else residual.reshape(-1, N))
@@ -143,7 +146,7 @@ class _LinearTrain(torch.autograd.Function):
             # The tensor itself: a view of it would be a new object over the same memory, which autograd
             # takes over as a leaf's .grad although the caller, or another leaf, still holds dy.
             dr = dy
-        return dx, dw, dbias, da, db, dr, None, None, None, None
+        return dx, dw, dbias, da, db, dr, None, None, None, None, None
 
 
 def _check_x(x: torch.Tensor, K: int, name: str) -> None:
@@ -193,7 +196,16 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
             raise RuntimeError(f"{name}: residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
     w_q, w_s, master = _fp8_weight(weight, name)
     return _LinearTrain.apply(x, master, bias, la, lb, residual, w_q, w_s, float(alpha),
-                              quant_mode)
+                              quant_mode, False)
+
+
+def frozen_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                  bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """The differentiable forward of :class:`BlockwiseFP8Linear`: its inference GEMM and quantiser,
+    so its output bits (but zeros for an all-zero 1x128 group of x), and gradients of x and the bias."""
+    _check_x(x, weight.shape[1], "BlockwiseFP8Linear")
+    return _LinearTrain.apply(x, None, bias, None, None, None, weight, weight_scale, 1.0,
+                              quant_mode_code() | L.QUANT_ZEROS, True)
 
 
 class _PreNormFeedForward(torch.autograd.Function):

@@ -98,3 +98,86 @@ def test_outputs_can_be_modified_in_place(cuda_device, lead, which):
     assert torch.equal(y, z) and y.shape == (*lead, skip.shape[-1])
     for p, q in zip(got, want):
         assert torch.equal(p, q)
+
+
+# ----------------------------------------------------------------------------- frozen linear
+def _linear(N, K, dev, seed, bias=True):
+    from ltx_kernels.blockwise import BlockwiseFP8Linear
+    layer = BlockwiseFP8Linear(K, N, bias=bias, device=dev)
+    layer.weight.data, layer.weight_scale.data = _weight(N, K, dev, seed)
+    if bias:
+        layer.bias.data = 0.1 * torch.randn(N, generator=gen(seed + 1)).to(dev)
+    return layer
+
+
+def _lora(N, K, r, dev, seed):
+    from ltx_kernels.blockwise import BlockwiseFP8LoRALinear
+    layer = BlockwiseFP8LoRALinear(K, N, r, alpha=0.5, device=dev)
+    layer.weight.data, layer.weight_scale.data = _weight(N, K, dev, seed)
+    layer.bias.data.zero_()
+    layer.lora_A.data = _bf16(r, K, seed=seed + 1, scale=K ** -0.5).to(dev)
+    layer.lora_B.data = _bf16(N, r, seed=seed + 2, scale=r ** -0.5).to(dev)
+    layer.lora_A.requires_grad_()
+    layer.lora_B.requires_grad_()
+    return layer
+
+
+@pytest.mark.parametrize("mode", ["triton", "torch"])
+@pytest.mark.parametrize("lead,bias", [((2, 65), True), ((1, 1), False), ((3, 100), True)])
+def test_gradient_through_a_frozen_linear(cuda_device, lead, bias, mode):
+    """An adapter below a frozen linear gets the gradient that float64 autograd gives; the
+    linear's output keeps its bits; its own parameters get none."""
+    from ltx_kernels.blockwise import functional
+    old = functional.get_quant_mode()
+    functional.set_quant_mode(mode)
+    try:
+        d, k, n, r = 256, 384, 256, 16
+        low, top = _lora(k, d, r, cuda_device, 61), _linear(n, k, cuda_device, 64, bias)
+        M = lead[0] * lead[1]
+        x = tokens(M, d, 66).view(*lead, d).to(cuda_device)
+        dy = (grads(M, n, 67).view(*lead, n) * 1e3).to(cuda_device)
+        h = low(x)
+        y = top(h)
+        with torch.no_grad():
+            assert torch.equal(y, top(h)) and torch.equal(y, top(low(x)))
+        assert y.requires_grad and y.shape == (*lead, n)
+        got = torch.autograd.grad(y, (low.lora_A, low.lora_B, h), dy)
+        assert top.weight.grad is None
+        p = [t.detach().double().requires_grad_() for t in (low.lora_A, low.lora_B)]
+        h64 = x.double() @ dequant_weight64(low.weight, low.weight_scale).t() + 0.5 * (x.double() @ p[0].t()) @ p[1].t()
+        y64 = h64 @ dequant_weight64(top.weight, top.weight_scale).t()
+        ref = torch.autograd.grad(y64, (*p, h64), dy.double())
+        # dy's 8-bit rounding for h; x's besides for A; bf16 roundings
+        for name, e, g, t in zip(("A", "B", "h"), (2, 1, 1), got, ref):
+            assert _rel(g, t) <= e * E4M3_RMS + 4 * 2 ** -8, (name, _rel(g, t))
+    finally:
+        functional.set_quant_mode(old)
+
+
+def test_frozen_linear_with_padded_tokens(cuda_device):
+    """All-zero tokens count as zeros where gradients flow (NaN without), so that they do not reach
+    the gradients of the others; a trainable bias gets its gradient."""
+    lin = _linear(256, 128, cuda_device, 81, bias=False)
+    x = _leaf(tokens(20, 128, 87, zero_rows=(3, 19)).view(1, 20, 128), cuda_device)
+    y = lin(x)
+    dy = (grads(20, 256, 88, zero_rows=(3, 19)).view(1, 20, 256) * 1e3).to(cuda_device)
+    (g,) = torch.autograd.grad(y, x, dy)
+    assert torch.isfinite(y).all() and torch.isfinite(g).all() and (y[0, 3] == 0).all() and (g[0, 3] == 0).all()
+    lin = _linear(256, 128, cuda_device, 89)
+    lin.bias.requires_grad_()
+    y = lin(x.detach()[:, 4:10])
+    y.backward(torch.ones_like(y))
+    assert torch.equal(lin.bias.grad, torch.full((256,), 6.0, device=cuda_device))
+
+
+def test_frozen_linear_takes_what_it_took(cuda_device):
+    """Quantised inputs, inputs without a gradient and no-grad calls run as before."""
+    from ltx_kernels.blockwise.functional import blockwise_quantize_triton
+    lin = _linear(256, 128, cuda_device, 91)
+    x = tokens(20, 128, 96).view(1, 20, 128).to(cuda_device)
+    y = lin(x)
+    assert not y.requires_grad
+    assert torch.equal(lin(blockwise_quantize_triton(x)), y)
+    with torch.no_grad():
+        z = lin(x.clone().requires_grad_())
+    assert torch.equal(z, y) and not z.requires_grad
