@@ -41,8 +41,9 @@ extern "C" {
 #define LTXFP8_QUANT_FINITE 2 /* scale = max(amax, 448 * 2^-126) / 448, code = e4m3(x / scale), within 1 ulp: an all-zero
                                  group gets zero codes (the modes above give NaN there).  ltxfp8_quantize_1x128 only;
                                  the residual-path operators at the end of this file always quantise this way */
-#define LTXFP8_QUANT_ZEROS 4  /* added to _TORCH or _TRITON in ltxfp8_quantize_1x128: the same codes and scales, but a
-                                 group whose s overflows (all zeros) gets zero codes and scale 0 instead of NaN */
+#define LTXFP8_QUANT_ZEROS 4  /* added to _TORCH or _TRITON in ltxfp8_quantize_1x128 and ltxfp8_gelu_tanh_quantize_1x128:
+                                 the same codes and scales, but a group whose s overflows (all zeros, or below
+                                 2^-119) gets zero codes and scale 0 instead of NaN */
 
 /* Input dtypes for ltxfp8_quantize_weight_128x128. */
 #define LTXFP8_DTYPE_F32 0
@@ -190,7 +191,8 @@ int ltxfp8_gelu_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld
  * Replaces the reference FFN's unfused chain after the up projection: F.gelu
  * (ltx-core/src/ltx_core/model/transformer/gelu_approx.py:10) on the bf16 GEMM output,
  * then blockwise::quantize in the down projection (ltx-kernels/.../linear.py:91-93).
- * Codes and scales equal ltxfp8_quantize_1x128 applied to torch's GELU output.
+ * Codes and scales equal ltxfp8_quantize_1x128 applied to torch's GELU output; flags:
+ * LTXFP8_QUANT_TORCH or _TRITON, with or without _ZEROS.
  */
 int ltxfp8_gelu_tanh_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, void* q, int64_t q_ld,
                                     float* sfa, int64_t sfa_ld, int flags, void* stream);

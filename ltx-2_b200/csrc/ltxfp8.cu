@@ -928,7 +928,9 @@ int ltxfp8_gelu_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld
 int ltxfp8_gelu_tanh_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t x_ld, void* q, int64_t q_ld,
                                     float* sfa, int64_t sfa_ld, int flags, void* stream) {
   if (M < 0 || K <= 0 || K % 128 != 0) return fail(LTXFP8_ERR_UNSUPPORTED_SHAPE, "gelu_tanh_quantize: need K %% 128 == 0, K > 0, M >= 0 (M=%lld K=%lld)", (long long)M, (long long)K);
-  if (flags != LTXFP8_QUANT_TORCH && flags != LTXFP8_QUANT_TRITON) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gelu_tanh_quantize: unknown mode %d", flags);
+  const int mode = flags & ~LTXFP8_QUANT_ZEROS;
+  const bool zeros = (flags & LTXFP8_QUANT_ZEROS) != 0;
+  if (mode != LTXFP8_QUANT_TORCH && mode != LTXFP8_QUANT_TRITON) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gelu_tanh_quantize: unknown mode %d", flags);
   if (M == 0) return LTXFP8_OK;
   if (!x || !q || !sfa) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gelu_tanh_quantize: null pointer");
   if (x_ld < K || q_ld < K || sfa_ld < M) return fail(LTXFP8_ERR_INVALID_ARGUMENT, "gelu_tanh_quantize: leading dimension too small");
@@ -954,10 +956,10 @@ int ltxfp8_gelu_tanh_quantize_1x128(const void* x, int64_t M, int64_t K, int64_t
   auto s = static_cast<cudaStream_t>(stream);
   const auto* xb = static_cast<const __nv_bfloat16*>(x);
   auto* qb = static_cast<uint8_t*>(q);
-  if (flags == LTXFP8_QUANT_TRITON)
-    gelu_tanh_quant_kernel<kQuantTriton><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
-  else
-    gelu_tanh_quant_kernel<kQuantTorch><<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
+  auto kern = mode == LTXFP8_QUANT_TRITON
+                  ? (zeros ? gelu_tanh_quant_kernel<kQuantTriton, true> : gelu_tanh_quant_kernel<kQuantTriton>)
+                  : (zeros ? gelu_tanh_quant_kernel<kQuantTorch, true> : gelu_tanh_quant_kernel<kQuantTorch>);
+  kern<<<grid, 256, 0, s>>>(xb, x_ld, M, KB, qb, q_ld, sfa, sfa_ld);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "gelu_tanh_quantize launch");
   return LTXFP8_OK;

@@ -109,9 +109,10 @@ __global__ void __launch_bounds__(256) quant_act_1x128_kernel(const __nv_bfloat1
 // applied to torch's bf16 GELU output.  A persistent grid: every CTA fills the 10.5 KB
 // GELU table once, then walks units of 16 rows x kQuantGroupsPerThread groups, groups
 // fastest (consecutive CTAs read consecutive bytes of the same rows).
+// kZeros: as quant_act_1x128_kernel's.
 constexpr int kGeluQuantGroups = 4;  // 1x128 groups per thread and unit
 
-template <int kMode>
+template <int kMode, bool kZeros = false>
 __global__ void __launch_bounds__(256) gelu_tanh_quant_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_ld,
                                                               int64_t M, int64_t KB, uint8_t* __restrict__ q,
                                                               int64_t q_ld, float* __restrict__ sfa,
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(256) gelu_tanh_quant_kernel(const __nv_bfloat1
       }
       float s, inv;
       group_scale<kMode>(amax, s, inv);
+      if (kZeros && isinf(s)) s = inv = 0.0f;
       const bool in_range = (kMode == kQuantTriton) || isfinite(s);
       uint32_t w[2];
 #pragma unroll

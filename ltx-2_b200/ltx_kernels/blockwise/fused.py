@@ -51,6 +51,7 @@ def fp8_linear(x: Activation, weight: torch.Tensor, weight_scale: torch.Tensor, 
     ``gelu=True`` is torch's GELU-tanh (the reference applies ``F.gelu(approximate="tanh")``
     to the bf16 output, gelu_approx.py:10); the input quantisation and the requantisation
     use the arithmetic of ``functional.set_quant_mode`` (default: the reference's GPU kernels).
+    The result carries no gradient: :func:`training.fp8_linear_train` is the differentiable linear.
     """
     ax = lb = None
     alpha = 1.0
@@ -73,7 +74,11 @@ def fp8_linear(x: Activation, weight: torch.Tensor, weight_scale: torch.Tensor, 
 class BlockwiseFP8FeedForward(nn.Module):
     """FFN: up projection, torch's GELU-tanh + 1x128 requantisation of the hidden state,
     down projection.  ``fused_epilogue``: GELU and requant inside the up projection's
-    GEMM epilogue instead of a separate streaming pass (same results)."""
+    GEMM epilogue instead of a separate streaming pass (same results).
+
+    Where gradients are enabled and the input or a bias requires one, the forward is differentiable
+    (:func:`training.frozen_feed_forward`): the same output, but an all-zero 1x128 group of the input or of
+    the hidden state, NaN otherwise, counts as zeros; the hidden state is kept in 8 bits."""
 
     def __init__(self, dim: int, dim_out: int, mult: int = 4, bias: bool = True, device=None,
                  fused_epilogue: bool = False):
@@ -93,6 +98,9 @@ class BlockwiseFP8FeedForward(nn.Module):
         return ff
 
     def forward(self, x: Activation) -> torch.Tensor:
+        if wants_gradient(x, self.proj_in.bias, self.proj_out.bias):
+            from .training import frozen_feed_forward
+            return frozen_feed_forward(x, self.proj_in, self.proj_out)
         if self.fused_epilogue:
             _, hq, hs = fp8_linear(x, self.proj_in.weight, self.proj_in.weight_scale, self.proj_in.bias,
                                    gelu=True, requant=True, write_d=False)

@@ -208,6 +208,47 @@ def frozen_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
                               quant_mode_code() | L.QUANT_ZEROS, True)
 
 
+class _FrozenFeedForward(torch.autograd.Function):
+    """The differentiable forward of BlockwiseFP8FeedForward: its quantisers and GEMMs, and 8-bit
+    codes of the hidden state for the activation's gradient."""
+
+    @staticmethod
+    def forward(ctx, x, b1, b2, w1, s1, w2, s2, quant_mode):
+        _check_capture("BlockwiseFP8FeedForward", x, b1, b2)
+        q, s = ops.quantize_1x128(_rows(x, x.shape[-1]), quant_mode)
+        z = ops.gemm(q, s, w1, s1, b1)
+        yq, ys = ops.gelu_tanh_quantize_1x128(z, quant_mode)
+        out, rows = _empty_output(x, w2.shape[0])
+        ops.gemm(yq, ys, w2, s2, b2, out=rows)
+        need_x, need_b1, _ = ctx.needs_input_grad[:3]
+        zq, zs = ops.quantize_1x128(z, L.QUANT_FINITE) if need_x or need_b1 else (None, None)
+        ctx.save_for_backward(zq, zs, w1, s1, w2, s2)
+        ctx.shape = x.shape
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        zq, zs, w1, s1, w2, s2 = ctx.saved_tensors
+        need_x, need_b1, need_b2 = ctx.needs_input_grad[:3]
+        g = _bf16_grad(dout, w2.shape[0])
+        dx = db1 = None
+        if need_x or need_b1:
+            _, dzq, dzs, db1 = ops.act_backward(_dgrad(g, w2, s2), zq, zs, "gelu_tanh", quantize=need_x, dbias=need_b1)
+            if need_x:
+                w1t, s1t = ops.transpose_weight_128x128(w1, s1)
+                dx = ops.gemm(dzq, dzs, w1t, s1t).view(ctx.shape)
+        return dx, db1, _column_sum(g) if need_b2 else None, None, None, None, None, None
+
+
+def frozen_feed_forward(x: torch.Tensor, up: BlockwiseFP8Linear, down: BlockwiseFP8Linear) -> torch.Tensor:
+    """The differentiable forward of :class:`BlockwiseFP8FeedForward`: the same output bits (but zeros
+    for an all-zero 1x128 group of x or of the hidden state), and gradients of x and the biases."""
+    _check_x(x, up.weight.shape[1], "BlockwiseFP8FeedForward")
+    return _FrozenFeedForward.apply(x, up.bias, down.bias, up.weight, up.weight_scale, down.weight, down.weight_scale,
+                                    quant_mode_code() | L.QUANT_ZEROS)
+
+
 class _PreNormFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, norm_weight, m1, b1, m2, b2, w1, s1, w2, s2, activation, eps, train):

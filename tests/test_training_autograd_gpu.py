@@ -181,3 +181,93 @@ def test_frozen_linear_takes_what_it_took(cuda_device):
     with torch.no_grad():
         z = lin(x.clone().requires_grad_())
     assert torch.equal(z, y) and not z.requires_grad
+
+
+# ----------------------------------------------------------------------------- frozen feed-forward
+@pytest.mark.parametrize("mode", ["triton", "torch"])
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("lead,bias", [((2, 65), True), ((1, 1), False), ((400,), True)])
+def test_gradient_through_a_frozen_feed_forward(cuda_device, lead, bias, fused, mode):
+    from ltx_kernels.blockwise import BlockwiseFP8FeedForward, functional
+    old = functional.get_quant_mode()
+    functional.set_quant_mode(mode)
+    try:
+        d, inner, n, r = 256, 512, 384, 16
+        low = _lora(d, d, r, cuda_device, 71)
+        ff = BlockwiseFP8FeedForward.from_linears(_linear(inner, d, cuda_device, 74, bias),
+                                                  _linear(n, inner, cuda_device, 76, bias))
+        ff.fused_epilogue = fused
+        M = 1
+        for i in lead:
+            M *= i
+        x = tokens(M, d, 78).view(*lead, d).to(cuda_device)
+        dy = (grads(M, n, 79).view(*lead, n) * 1e3).to(cuda_device)
+        h = low(x)
+        y = ff(h)
+        with torch.no_grad():
+            assert torch.equal(y, ff(h))
+        assert y.requires_grad and y.shape == (*lead, n)
+        got = torch.autograd.grad(y, (low.lora_A, low.lora_B, h), dy)
+        p = [t.detach().double().requires_grad_() for t in (low.lora_A, low.lora_B)]
+        h64 = x.double() @ dequant_weight64(low.weight, low.weight_scale).t() + 0.5 * (x.double() @ p[0].t()) @ p[1].t()
+        b1, b2 = ((l.bias.double() if bias else 0.0) for l in (ff.proj_in, ff.proj_out))
+        z64 = h64 @ dequant_weight64(ff.proj_in.weight, ff.proj_in.weight_scale).t() + b1
+        y64 = act64(z64, "gelu_tanh") @ dequant_weight64(ff.proj_out.weight, ff.proj_out.weight_scale).t() + b2
+        ref = torch.autograd.grad(y64, (*p, h64), dy.double())
+        # h: dy, dz and z's three (its checkpoint and h's codes below it, slope |z act''| <= 1.5 of act');
+        # A: x's besides
+        for name, e, g, t in zip(("A", "B", "h"), (6, 5, 5), got, ref):
+            assert _rel(g, t) <= e * E4M3_RMS + 4 * 2 ** -8, (name, _rel(g, t))
+        assert _rel(y, y64) <= 2.5 * E4M3_RMS + 2 ** -8
+    finally:
+        functional.set_quant_mode(old)
+
+
+def test_frozen_feed_forward_with_padded_tokens(cuda_device):
+    from ltx_kernels.blockwise import BlockwiseFP8FeedForward
+    ff = BlockwiseFP8FeedForward.from_linears(_linear(512, 128, cuda_device, 83, bias=False),
+                                              _linear(128, 512, cuda_device, 85, bias=False))
+    x = _leaf(tokens(20, 128, 87, zero_rows=(3, 19)).view(1, 20, 128), cuda_device)
+    y = ff(x)
+    dy = (grads(20, 128, 88, zero_rows=(3, 19)).view(1, 20, 128) * 1e3).to(cuda_device)
+    (g,) = torch.autograd.grad(y, x, dy)
+    assert torch.isfinite(y).all() and torch.isfinite(g).all() and (y[0, 3] == 0).all() and (g[0, 3] == 0).all()
+    ff.proj_in.register_parameter("bias", torch.nn.Parameter(torch.zeros(512, device=cuda_device)))
+    ff.proj_out.register_parameter("bias", torch.nn.Parameter(torch.zeros(128, device=cuda_device)))
+    y = ff(x.detach()[:, 4:10])
+    y.backward(torch.ones_like(y))
+    assert torch.equal(ff.proj_out.bias.grad, torch.full((128,), 6.0, device=cuda_device))
+    assert torch.isfinite(ff.proj_in.bias.grad).all() and (ff.proj_in.bias.grad != 0).any()
+
+
+def test_frozen_feed_forward_takes_what_it_took(cuda_device):
+    from ltx_kernels.blockwise import BlockwiseFP8FeedForward
+    from ltx_kernels.blockwise.functional import blockwise_quantize_triton
+    ff = BlockwiseFP8FeedForward.from_linears(_linear(512, 128, cuda_device, 92), _linear(128, 512, cuda_device, 94))
+    x = tokens(20, 128, 96).view(1, 20, 128).to(cuda_device)
+    y = ff(x)
+    assert not y.requires_grad
+    assert torch.equal(ff(blockwise_quantize_triton(x)), y)
+    with torch.no_grad():
+        z = ff(x.clone().requires_grad_())
+    assert torch.equal(z, y) and not z.requires_grad
+    empty = ff(x[:, :0].clone().requires_grad_())
+    assert empty.shape == (1, 0, 128)
+    assert torch.autograd.grad(empty.sum(), empty, allow_unused=True)[0] is not None
+
+
+def test_gelu_quantiser_without_nan(cuda_device):
+    """QUANT_ZEROS in the GELU quantiser: the same bytes but for groups without a finite scale."""
+    from ltx_kernels import _lib as L
+    from ltx_kernels.blockwise import ops
+    x = tokens(67, 384, 107).to(cuda_device)
+    x[3], x[5, 128:256], x[7, :128], x[9, 0] = 0, -40, -1e-37, float("nan")
+    lost = torch.zeros(67, 3, dtype=torch.bool, device=cuda_device)
+    lost[3], lost[5, 1], lost[7, 0] = True, True, True
+    for mode in (L.QUANT_TORCH, L.QUANT_TRITON):
+        (q0, s0), (q1, s1) = (ops.gelu_tanh_quantize_1x128(x, m) for m in (mode, mode | L.QUANT_ZEROS))
+        a, b = q0.view(torch.uint8).view(67, 3, 128), q1.view(torch.uint8).view(67, 3, 128)
+        assert torch.equal(a[~lost], b[~lost]) and (b[lost] & 0x7F == 0).all()
+        assert torch.equal(s0[~lost].nan_to_num(7.0), s1[~lost].nan_to_num(7.0)) and (s1[lost] == 0).all()
+    with pytest.raises(RuntimeError, match="unknown mode"):
+        ops.gelu_tanh_quantize_1x128(x, L.QUANT_FINITE)
