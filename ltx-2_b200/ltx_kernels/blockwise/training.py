@@ -64,11 +64,11 @@ def _empty_output(x: torch.Tensor, N: int) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def _check_capture(name: str, *leaves: Optional[torch.Tensor]) -> None:
-    """Refuse, while a CUDA graph is captured, leaves whose gradient node was made on the default
-    stream and is still alive (an earlier eager result that has not been released): autograd
-    would run that node on the default stream, which a capture forbids, and the error ends the
-    process from its backward thread."""
-    if torch.cuda.is_current_stream_capturing():
+    """Refuse, while a CUDA graph is captured with gradients enabled, leaves whose gradient node was
+    made on the default stream and is still alive (an earlier eager result that has not been
+    released): autograd would run that node on the default stream, which a capture forbids, and the
+    error ends the process from its backward thread."""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
         L.binding().check_capture(name, [t for t in leaves if t is not None and t.is_leaf and t.requires_grad])
 
 
@@ -90,7 +90,6 @@ def _bf16_grad(g: torch.Tensor, width: int) -> torch.Tensor:
 class _LinearTrain(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, master, bias, lora_a, lora_b, residual, w_q, w_s, alpha, quant_mode, plain):
-        _check_capture("fp8_linear_train", x, master, bias, lora_a, lora_b, residual)
         K, N = x.shape[-1], w_q.shape[0]
         x2 = _rows(x, K)
         q, s = ops.quantize_1x128(x2, quant_mode)
@@ -194,6 +193,7 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
         _check_x(residual, N, f"{name}: residual")
         if residual.shape[:-1] != x.shape[:-1]:
             raise RuntimeError(f"{name}: residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+    _check_capture(name, x, None if isinstance(weight, (tuple, list)) else weight, bias, la, lb, residual)
     w_q, w_s, master = _fp8_weight(weight, name)
     return _LinearTrain.apply(x, master, bias, la, lb, residual, w_q, w_s, float(alpha),
                               quant_mode, False)
@@ -204,6 +204,7 @@ def frozen_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Ten
     """The differentiable forward of :class:`BlockwiseFP8Linear`: its inference GEMM and quantiser,
     so its output bits (but zeros for an all-zero 1x128 group of x), and gradients of x and the bias."""
     _check_x(x, weight.shape[1], "BlockwiseFP8Linear")
+    _check_capture("BlockwiseFP8Linear", x, bias)
     return _LinearTrain.apply(x, None, bias, None, None, None, weight, weight_scale, 1.0,
                               quant_mode_code() | L.QUANT_ZEROS, True)
 
@@ -214,7 +215,6 @@ class _FrozenFeedForward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, b1, b2, w1, s1, w2, s2, quant_mode):
-        _check_capture("BlockwiseFP8FeedForward", x, b1, b2)
         q, s = ops.quantize_1x128(_rows(x, x.shape[-1]), quant_mode)
         z = ops.gemm(q, s, w1, s1, b1)
         yq, ys = ops.gelu_tanh_quantize_1x128(z, quant_mode)
@@ -245,6 +245,7 @@ def frozen_feed_forward(x: torch.Tensor, up: BlockwiseFP8Linear, down: Blockwise
     """The differentiable forward of :class:`BlockwiseFP8FeedForward`: the same output bits (but zeros
     for an all-zero 1x128 group of x or of the hidden state), and gradients of x and the biases."""
     _check_x(x, up.weight.shape[1], "BlockwiseFP8FeedForward")
+    _check_capture("BlockwiseFP8FeedForward", x, up.bias, down.bias)
     return _FrozenFeedForward.apply(x, up.bias, down.bias, up.weight, up.weight_scale, down.weight, down.weight_scale,
                                     quant_mode_code() | L.QUANT_ZEROS)
 
@@ -252,7 +253,6 @@ def frozen_feed_forward(x: torch.Tensor, up: BlockwiseFP8Linear, down: Blockwise
 class _PreNormFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, norm_weight, m1, b1, m2, b2, w1, s1, w2, s2, activation, eps, train):
-        _check_capture("pre_norm_feed_forward", x, residual, norm_weight, m1, b1, m2, b2)
         K = x.shape[-1]
         x2 = x.reshape(-1, K)
         r2 = None if residual is None else residual.reshape(-1, K)
@@ -326,6 +326,8 @@ def pre_norm_feed_forward(x: torch.Tensor, w1: Weight, w2: Weight, *, residual: 
             raise RuntimeError(f"{name}: residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
     _check_bias(b1, inner, f"{name}: b1")
     _check_bias(b2, d, f"{name}: b2")
+    _check_capture(name, x, residual, norm_weight, b1, b2,
+                   *(w for w in (w1, w2) if not isinstance(w, (tuple, list))))
     q1, s1, m1 = _fp8_weight(w1, f"{name}: w1")
     q2, s2, m2 = _fp8_weight(w2, f"{name}: w2")
     # What only the backward pass reads is not written when no gradient is wanted.

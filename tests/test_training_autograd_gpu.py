@@ -100,6 +100,32 @@ def test_outputs_can_be_modified_in_place(cuda_device, lead, which):
         assert torch.equal(p, q)
 
 
+# ----------------------------------------------------------------------------- captures
+def test_inference_capture_beside_a_living_eager_result(cuda_device):
+    """Without gradients nothing of a capture reaches a leaf's gradient node: evaluating a block in
+    a CUDA graph while a training step's loss is alive."""
+    from ltx_kernels.blockwise import fp8_linear_train, pre_norm_feed_forward
+    w1, w2 = _weight(256, 128, cuda_device, 41), _weight(128, 256, cuda_device, 42)
+    nw = _leaf(torch.ones(128), cuda_device)
+    m = _leaf(torch.randn(128, 128, generator=gen(43)), cuda_device)
+    x = tokens(16, 128, 44).to(cuda_device)
+    y = fp8_linear_train(pre_norm_feed_forward(x, w1, w2, norm_weight=nw), m)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    refused = None
+    with torch.no_grad(), torch.cuda.graph(graph):
+        try:
+            z = fp8_linear_train(pre_norm_feed_forward(x, w1, w2, norm_weight=nw), m)
+        except RuntimeError as e:
+            refused = e
+    assert refused is None, refused
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(z, y) and not z.requires_grad
+    for g in torch.autograd.grad(y, (nw, m), torch.ones_like(y)):
+        assert torch.isfinite(g).all()
+
+
 # ----------------------------------------------------------------------------- frozen linear
 def _linear(N, K, dev, seed, bias=True):
     from ltx_kernels.blockwise import BlockwiseFP8Linear
@@ -254,8 +280,6 @@ def test_frozen_feed_forward_takes_what_it_took(cuda_device):
     empty = ff(x[:, :0].clone().requires_grad_())
     assert empty.shape == (1, 0, 128)
     assert torch.autograd.grad(empty.sum(), empty, allow_unused=True)[0] is not None
-
-
 def test_gelu_quantiser_without_nan(cuda_device):
     """QUANT_ZEROS in the GELU quantiser: the same bytes but for groups without a finite scale."""
     from ltx_kernels import _lib as L
