@@ -683,10 +683,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // Split-K reduction: out = epilogue( sum_split partial + bias ), summing each
 // tile's unit partials in split order (deterministic).  One half-warp per (tile
 // row, 128-column group): 16 lanes x 8 columns, so the 1x128 requantisation needs
-// no cross-row reduction.  Epilogue semantics are those of the GEMM kernel.
+// no cross-row reduction.  Epilogue semantics are those of the GEMM kernel.  `res` may be p.d.
 template <bool kGelu, bool kRequant, int kAct = -1>
 __global__ void __launch_bounds__(256)
-    splitk_reduce_kernel(const GemmParams p, const __nv_bfloat16* __restrict__ res, int64_t res_ld) {
+    splitk_reduce_kernel(const GemmParams p, const __nv_bfloat16* res, int64_t res_ld) {
   const int64_t total = static_cast<int64_t>(p.total_tiles) * kBM * 2;
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int l16 = threadIdx.x & 15;

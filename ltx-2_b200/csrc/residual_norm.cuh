@@ -381,10 +381,11 @@ __global__ void __launch_bounds__(norm_threads<kWarps>) rms_norm_bwd_kernel(cons
 // out[n] = sum over p of part[p, n], in the type of `out` (fp32 or bf16): a block sums 32
 // columns, its kColSumWarps warps every kColSumWarps-th partial row each, in a fixed order.
 // Latency-bound (296 rows at most of a norm: ten dependent loads a thread would be, in one batch
-// of loads here): 2.5 to 3 us with the launch, whose start overlaps the first kernel's end.
+// of loads here): 2.5 to 3 us with the launch, whose start overlaps the first kernel's end.  `part` is
+// not __restrict__: it is being written when this kernel starts.
 constexpr int kColSumWarps = 32;
 __global__ void __launch_bounds__(kColSumWarps * 32)
-    col_sum_kernel(const float* __restrict__ part, int parts, int N, void* out, bool out_f32) {
+    col_sum_kernel(const float* part, int parts, int N, void* out, bool out_f32) {
   __shared__ float red[kColSumWarps][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = blockIdx.x * 32 + lane;
