@@ -52,29 +52,40 @@ def needs_build() -> bool:
 
 
 def build_binding(force: bool = False) -> str:
-    src = os.path.join(SRC_DIR, "torch_binding.cpp")
-    if not force and not _stale(BINDING_PATH, [src, os.path.join(INCLUDE, "ltxfp8.h")]):
-        return BINDING_PATH
+    import sys
     import sysconfig
 
     import torch
 
+    src = os.path.join(SRC_DIR, "torch_binding.cpp")
     root = os.path.dirname(torch.__file__)
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     tmp = os.path.join(LIB_DIR, "_ltxfp8_torch.tmp.so")
     # The system's g++, not $CXX: a compiler that links its own libstdc++ statically puts a second
     # C++ runtime beside torch's, and an exception that crosses them ends the process.
-    subprocess.check_call([
+    cmd = [
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f'-DLTXFP8_TORCH_VERSION="{torch.__version__}"',
         "-I" + INCLUDE, "-isystem", os.path.join(root, "include"),
         "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
         "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
         src, "-o", tmp, "-L" + LIB_DIR, "-l:libltxfp8.so", "-L" + os.path.join(root, "lib"),
-        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+        "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    # What it was built with, beside it: file times do not tell that torch or Python has changed.
+    # (Without the folders, which differ between machines that share the tree.)
+    record = BINDING_PATH + ".built_with"
+    key = f"torch {torch.__version__}, python {sys.version.split()[0]}, {' '.join(cmd[1:8])}"
+    if not force and not _stale(BINDING_PATH, [src, os.path.join(INCLUDE, "ltxfp8.h")]) and os.path.exists(record):
+        with open(record) as f:
+            if f.read() == key:
+                return BINDING_PATH
+    subprocess.check_call(cmd)
     if b"libstdc++.so" not in subprocess.check_output(["readelf", "-d", tmp]):
         raise RuntimeError("the tensor-level binding must share torch's C++ runtime (libstdc++.so), but g++ linked its own")
     os.replace(tmp, BINDING_PATH)
+    with open(record, "w") as f:
+        f.write(key)
     return BINDING_PATH
 
 

@@ -456,4 +456,9 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ltxfp8_torch", nullptr, -1, kMet
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__ltxfp8_torch(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__ltxfp8_torch(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  // The torch it was compiled against, compared with the running one by the loader.
+  if (m && PyModule_AddStringConstant(m, "torch_version", LTXFP8_TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -163,6 +163,15 @@ def load(path: str | None = None):
 _binding = None
 
 
+def check_binding(mod) -> None:
+    """Refuse a binding compiled against another torch: its calls into torch's C++ interface may
+    not fit this one."""
+    import torch
+    if mod.torch_version != torch.__version__:
+        raise ImportError(f"{BINDING_PATH} was built for torch {mod.torch_version}, this is {torch.__version__}: "
+                          "build it again (python ltx-2_b200/build.py)")
+
+
 def binding():
     """Load (once) and return the compiled tensor-level calls (csrc/torch_binding.cpp)."""
     global _binding
@@ -181,6 +190,7 @@ def binding():
             spec = importlib.util.spec_from_file_location("_ltxfp8_torch", BINDING_PATH)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
+            check_binding(mod)
             mod.set_check(check)
             _binding = mod
     return _binding
