@@ -168,8 +168,9 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
     ``x`` bf16 ``[..., K]``.  ``weight`` is a frozen ``(e4m3 [N, K], fp32 scales [N/128, K/128])``
     pair or a bf16 / fp32 master weight ``[N, K]``, which is quantised for this call and
     receives the gradient ``dY^T x~``.  ``bias`` fp32 ``[N]``.  ``lora = (A [r, K], B [N, r],
-    alpha)``, r a multiple of 16 up to 256, used in bf16.  ``residual`` bf16 of the output's shape,
-    added in the GEMM's epilogue (after the LoRA term when there is one).
+    alpha)``, r a multiple of 16 up to 256, used in bf16.  ``residual`` bf16 of the output's shape:
+    added in the GEMM's epilogue before the only rounding; with ``lora`` by an addition of its own to
+    the linear's bf16 result, a second rounding.
 
     What the backward pass keeps of ``x`` is its e4m3 codes and scales (``x~``, where the weight
     or A wants a gradient), and with LoRA ``x A^T``; the weight is not copied.  The gradient of

@@ -100,6 +100,34 @@ def test_outputs_can_be_modified_in_place(cuda_device, lead, which):
         assert torch.equal(p, q)
 
 
+# ----------------------------------------------------------------------------- LoRA and residual
+@pytest.mark.parametrize("lead", [(130,), (2, 65)])
+def test_lora_with_residual(cuda_device, lead):
+    """The linear with LoRA is rounded to bf16, then the residual added and rounded again; the
+    gradients are the linear's, and the output's own gradient for the residual."""
+    from ltx_kernels.blockwise import fp8_linear_train
+    M, K, N, r = 130, 256, 384, 32
+    w, s = _weight(N, K, cuda_device, 31)
+    x, res = _leaf(tokens(M, K, 32).view(*lead, K), cuda_device), _leaf(tokens(M, N, 33).view(*lead, N), cuda_device)
+    a, b = _leaf(_bf16(r, K, seed=34, scale=K ** -0.5), cuda_device), _leaf(_bf16(N, r, seed=35, scale=r ** -0.5),
+                                                                              cuda_device)
+    bias = _leaf(0.1 * torch.randn(N, generator=gen(36)), cuda_device)
+    dy = (grads(M, N, 37).view(*lead, N) * 1e3).to(cuda_device)
+    y = fp8_linear_train(x, (w, s), bias, lora=(a, b, 0.5), residual=res)
+    got = torch.autograd.grad(y, (x, a, b, bias, res), dy)
+    y0 = fp8_linear_train(x, (w, s), bias, lora=(a, b, 0.5))
+    assert torch.equal(y, y0 + res)
+    for p, q in zip(got, (*torch.autograd.grad(y0, (x, a, b, bias), dy), dy)):
+        assert torch.equal(p, q) and p.shape == q.shape
+    p = [t.detach().double().requires_grad_() for t in (x, a, b, bias, res)]
+    y64 = p[0] @ dequant_weight64(w, s).t() + 0.5 * (p[0] @ p[1].t()) @ p[2].t() + p[3] + p[4]
+    ref = torch.autograd.grad(y64, p, dy.double())
+    # the output: x's 8-bit rounding, x A^T's and the two of the sum in bf16
+    assert _rel(y, y64) <= E4M3_RMS + 3 * 2 ** -8
+    for name, n, g, t in zip(("x", "A", "B", "bias", "residual"), (1, 1, 0, 0, 0), got, ref):
+        assert _rel(g, t) <= n * E4M3_RMS + 3 * 2 ** -8, (name, _rel(g, t))
+
+
 # ----------------------------------------------------------------------------- captures
 def test_inference_capture_beside_a_living_eager_result(cuda_device):
     """Without gradients nothing of a capture reaches a leaf's gradient node: evaluating a block in
