@@ -353,8 +353,9 @@ int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_
  * residual and no gain in its norms).  Quantised outputs use LTXFP8_QUANT_FINITE and the
  * layout of ltxfp8_quantize_1x128 with q_ld = the row length.  Row operands are bf16 with
  * 16-byte aligned rows (row strides in elements, multiples of 8); outputs are contiguous.
- * All arithmetic is fp32, each output rounded once; sums over tokens are taken in a fixed
- * order, so results repeat bit for bit on the same device.
+ * All arithmetic is fp32, each output rounded once (but for ltxfp8_wgrad, which rounds the
+ * expanded codes to bf16 as well); sums over tokens are taken in a fixed order, so results
+ * repeat bit for bit on the same device.
  */
 
 /*
@@ -418,8 +419,8 @@ int ltxfp8_act_backward_workspace_bytes(int64_t M, int64_t N, size_t* bytes);
 /*
  * Weight gradient: out[n, k] = bf16( alpha * sum over m of g[m, n] * x[m, k] ).
  * g bf16 [M, N] (N % 16 == 0); x [M, K] (K % 128 == 0) either e4m3 codes with scales xs
- * (element (m, kb) at xs[kb * xs_ld + m]; x_ld in bytes, a multiple of 16), each value
- * expanded to bf16, or bf16 when xs is NULL.  transposed: out is [K, N] instead of [N, K].
+ * (element (m, kb) at xs[kb * xs_ld + m]; x_ld in bytes, a multiple of 16), each code * scale
+ * rounded to bf16 on the way into the tensor core, or bf16 when xs is NULL.  transposed: out is [K, N] instead of [N, K].
  * Needs a workspace of ltxfp8_wgrad_workspace_bytes (0: none).  M == 0 gives zeros.
  */
 int ltxfp8_wgrad(const void* g, int64_t g_ld, const void* x, int64_t x_ld, const float* xs, int64_t xs_ld, float alpha,

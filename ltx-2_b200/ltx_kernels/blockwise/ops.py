@@ -563,7 +563,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     multiple of 128 up to 16384; ``weight`` is fp32 or bf16 ``[H]`` or None.  Returns
     ``(codes [M, H], scales (M, H/128), h, rstd [M])``, or with ``quantize=False``
     ``(y bf16 [M, H], h, rstd)``; ``h`` and ``rstd`` are what :func:`rms_norm_backward`
-    needs.  All-zero rows quantise to zero codes."""
+    needs.  All-zero rows quantise to zero codes (with ``eps`` 0 they have no norm: NaN)."""
     return L.binding().rms_norm_quantize(x, weight, residual, eps, quantize)
 
 
@@ -619,7 +619,10 @@ def wgrad_1x128(g: torch.Tensor, x_q: torch.Tensor, x_scales: torch.Tensor, *, a
 
     ``g`` bf16 [..., N] is the gradient of the layer's output (N a multiple of 16, so LoRA
     ranks fit), ``x_q``/``x_scales`` the input's e4m3 codes [..., K] and 1x128 scales, as the
-    forward GEMM read them.  Codes are expanded to bf16 on their way into the tensor core."""
+    forward GEMM read them.  Each code * scale is rounded to bf16 on its way into the tensor core
+    (2^-8 of it at most, a sixteenth of the code's own rounding), sums are fp32, the result is
+    rounded once: about a third more error than rounding the result alone (0.0022 against 0.0017 of
+    it in the root mean square)."""
     return L.binding().wgrad_1x128(g, x_q, x_scales, alpha, transposed)
 
 

@@ -174,8 +174,10 @@ def fp8_linear_train(x: torch.Tensor, weight: Weight, bias: Optional[torch.Tenso
 
     What the backward pass keeps of ``x`` is its e4m3 codes and scales (``x~``, where the weight
     or A wants a gradient), and with LoRA ``x A^T``; the weight is not copied.  The gradient of
-    ``x`` is a blockwise-FP8 GEMM of the quantised output gradient.  ``quant_mode``: of ``x``, as
-    ``ops.quantize_1x128`` takes it."""
+    ``x`` is a blockwise-FP8 GEMM of the quantised output gradient.  Gradients of a master weight and
+    of the LoRA factors are rounded to bf16, from fp32 sums over ``x~`` in bf16 (code * scale rounded
+    once), also where the parameter is fp32.  ``quant_mode``: of ``x``, as ``ops.quantize_1x128``
+    takes it."""
     name = "fp8_linear_train"
     shape = weight[0].shape if isinstance(weight, (tuple, list)) else weight.shape
     if len(shape) != 2:
@@ -311,7 +313,8 @@ def pre_norm_feed_forward(x: torch.Tensor, w1: Weight, w2: Weight, *, residual: 
     ``x``, ``residual`` bf16 ``[..., d]``; ``w1`` [inner, d] and ``w2`` [d, inner] each a frozen
     ``(e4m3, scales)`` pair or a bf16 / fp32 master weight that gets a gradient; ``norm_weight``
     fp32 or bf16 ``[d]``; ``b1``, ``b2`` fp32; ``activation`` ``"gelu_tanh"`` or ``"silu"``.
-    Differentiable in x, residual, norm_weight, master weights and biases.  The backward pass
+    Differentiable in x, residual, norm_weight, master weights (whose gradients are rounded to bf16, as
+    :func:`fp8_linear_train`'s) and biases.  The backward pass
     keeps h in bf16, the activation's input in 8 bits and, for the gradients of w1 and w2, the
     normalised input and the activation's output in 8 bits; without gradients nothing is kept
     and the activation's input is not quantised."""
