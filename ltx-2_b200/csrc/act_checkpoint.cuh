@@ -46,7 +46,7 @@ constexpr int kActSaveGroups = 32 * kActSaveUnroll;  // 1x128 groups of a 256-th
 // One pass, 8 lanes a group (its abs-max is three shuffles), two groups a thread in flight.  Without
 // a checkpoint it is an instantiation of its own: as a branch it cost 180 bytes of spills (113
 // against 71 us at 6144 x 16384).
-// Measured, GELU with the checkpoint at 6144 x 16384: 71 us, 5.8 TB/s; the floor is 63 us of
+// Measured, GELU with the checkpoint at 6144 x 16384: 72 us, 5.7 TB/s; the floor is 63 us of
 // traffic (4.06 bytes a value).  What it spends besides are instructions: 17 a value, two of them on
 // the exponential unit (exp2 and the reciprocal, 43 us of that unit alone); at a clock of 1.4 GHz
 // under the power cap the same launch takes 93 us.
@@ -112,7 +112,7 @@ struct ActBwdParams {
 // about 20 others a value) hides the loads only if many are in flight, so bulk copies bring
 // dy and the codes through a ring of shared-memory stages.  A stage is released by one
 // arrival per warp as soon as its values are in registers.
-// Measured with dz in both forms and dbias at 6143 x 16384: 107 us, 5.7 TB/s (floor 94 us of
+// Measured with dz in both forms and dbias at 6143 x 16384: 107 to 109 us, 5.6 TB/s (floor 94 us of
 // traffic); three stages (108 KB in flight on an SM) are best: two 109, four 109, six 111; loads to
 // registers alone took 134 us where the first ring took 122.
 // kDirect: a few rows (one share, so no partial sums and no second launch): the loads go straight

@@ -2,9 +2,9 @@
 //
 //   D[m, n] = bf16( act( sum_kb sfa[m,kb] sfb[n/128,kb] (A[m,kb] . W[n,kb]) + bias[n] ) + residual[m, n] )
 //
-// Bound by reading the weight once: 7 x 4096 x 4096 takes 10.2 us with the weight in memory (1.7 TB/s,
-// of which 3 us are a launch's; 256 blocks ask for their 64 KB each at once and wait for it once)
-// and 5.3 us with it in L2.  The tensor-core kernel's 128-row tiles leave it 144 busy
+// Bound by reading the weight once: 7 x 4096 x 4096 takes 6.6 us in a chain of launches over 1 GB of
+// weights (2.5 TB/s: 256 blocks ask for their 64 KB each at once and wait for it once), 5.1 us with
+// the weight in L2 and 9 to 10 us as a launch alone behind an L2 flush, its start included.  The tensor-core kernel's 128-row tiles leave it 144 busy
 // CTAs, a workspace of partial sums and a second launch; here a block owns 16 weight rows, each
 // of its 8 warps an eighth of their K blocks (consecutive, so that a row is read in long
 // stretches), and mma.sync m16n8k32 multiplies 16 weight rows by 8 tokens straight from registers:

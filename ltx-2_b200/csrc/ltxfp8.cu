@@ -1293,9 +1293,12 @@ int ltxfp8_lora_a(const void* x, const void* lora_a, void* ax, int64_t M, int64_
 
 // ----------------------------------------------------------------------------- residual epilogue
 // Where the weight-streaming kernel runs instead of the tensor-core one (and its split-K
-// reduction).  Measured, weight from memory, streaming / tensor-core: 8 tokens 4096 x 4096
-// 6.8 / 12.3 us, 16384 x 4096 18.7 / 24.4, 4096 x 16384 20.0 / 21.4; 16 tokens 4096 x 4096
-// 7.6 / 12.5, 16384 x 4096 24.6 / 23.7; 32 tokens 4096 x 4096 12.1 / 13.3, 16384 x 4096 42 / 24.
+// reduction).  Measured, streaming / tensor-core, launches one after the other over 1 GB of weights
+// in rotation (N x K): 8 tokens 1024 x 2048 3.8 / 8.1 us, 4096 x 4096 6.6 / 10.8, 16384 x 4096
+// 17.6 / 23.3, 4096 x 16384 19.1 / 19.4; 16 tokens 4096 x 4096 7.4 / 10.9, 8192 x 4096 13.0 / 14.5,
+// 16384 x 4096 23.8 / 23.2, 4096 x 16384 21.3 / 19.8 (9 tokens 20.8 / 19.4).  With the weight in L2:
+// 8 tokens 4096 x 4096 5.1 / 10.0, 4096 x 16384 12.7 / 14.7; 16 tokens 8192 x 4096 10.4 / 13.5.  A form
+// for 32 tokens gained 9 % at 4096 x 4096 (12.1 / 13.3), lost at 16384 x 4096 (42 / 24) and is not kept.
 static bool gemm_small_wins(int64_t M, int64_t N, int64_t K) {
   return M <= 8 || (M <= 16 && N * K <= (static_cast<int64_t>(1) << 25));
 }

@@ -13,10 +13,11 @@
 // it, each thread owning kChunks runs of 16 consecutive values (two 16-byte loads), so
 // 8 lanes hold one 1x128 group and its abs-max is three shuffles.  Every value is read once
 // and written once: the floor is memory traffic (7.03 bytes a value forward with a residual and
-// codes, 8 backward with dh).  Measured, tokens x width: forward 24576 x 4096 107 us (6.6 TB/s, the
-// measured copy rate), 1003 x 2048 without a residual 4.2 us, 8 x 4096 3.2 us (a launch); backward
-// with the gain's gradient 24576 x 4096 124 us (6.5 TB/s), 1003 x 2048 8.3 us, of which the sum
-// of the blocks' partial gains, a second launch, is 3.
+// codes, 8 backward with dh).  Measured, tokens x width, in a chain of launches over 600 MB of inputs in
+// rotation: forward 24576 x 4096 107 us (6.6 TB/s in a burst at 1965 MHz, a plain copy 6.5; 117 us in
+// calls that last, under the power cap), 1003 x 2048 without a residual 3.3 us, 8 x 4096 2.0 us (a
+// launch); backward with the gain's gradient 24576 x 4096 124 us (6.5 TB/s; 130 in calls that last),
+// 1003 x 2048 8.5 us, of which the sum of the blocks' partial gains, a second launch, is 3.
 #pragma once
 
 #include "quant.cuh"

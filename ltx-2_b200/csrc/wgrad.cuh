@@ -34,7 +34,9 @@
 // Measured, 2 M N K / time: 6144 x 4096 x 4096 151 us (1366 TFLOP/s, tensor pipe 86 % active; the
 // library's product of bf16 operands, without the expansion, takes 138), 24576 x 4096 x 4096 565 us
 // (1460 TFLOP/s).  For few columns of g (LoRA factors) the expansion bounds it, 16 codes a cycle
-// and SM: 6143 x 32 x 4096 15 us and 24576 x 128 x 4096 38, against 4 and 17 of traffic.
+// and SM, for many tokens: 24576 x 128 x 4096 takes 38 us against 17 of traffic, about 22 of them
+// expansion.  At 6143 x 32 x 4096 (15 us against 4) it is 11 stages of some 924 cycles a unit, 5 us; the
+// rest is fixed: launch, set-up and drain, the fp32 partials' way through memory, the second launch.
 // The summed axis is divided among `splits` units where the tiles alone would not fill the
 // GPU; those write fp32 partials that wgrad_reduce_kernel adds in split order.
 #pragma once
