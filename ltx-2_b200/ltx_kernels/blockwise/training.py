@@ -11,7 +11,9 @@ quantise to zeros here.
   train, or a bf16 / fp32 master weight that is quantised per call and gets a gradient;
 * :func:`pre_norm_feed_forward` -- a whole un-gated pre-norm block, ``h + W2 act(W1 norm(h))``
   with ``h = x + residual``, whose intermediate tensors are kept in 8 bits only;
-* :class:`BlockwiseFP8PreNormFeedForward` -- that block as a module.
+* :class:`BlockwiseFP8PreNormFeedForward` -- that block as a module;
+* :func:`frozen_linear`, :func:`frozen_feed_forward` -- what ``BlockwiseFP8Linear`` and
+  ``BlockwiseFP8FeedForward`` run where their input or a bias requires a gradient.
 
 No reference counterpart: the reference's blockwise linear is forward-only
 (ltx-kernels/src/ltx_kernels/blockwise/linear.py:82-104).

@@ -323,3 +323,30 @@ def test_gelu_quantiser_without_nan(cuda_device):
         assert torch.equal(s0[~lost].nan_to_num(7.0), s1[~lost].nan_to_num(7.0)) and (s1[lost] == 0).all()
     with pytest.raises(RuntimeError, match="unknown mode"):
         ops.gelu_tanh_quantize_1x128(x, L.QUANT_FINITE)
+
+
+def test_frozen_layers_in_a_cuda_graph(cuda_device):
+    """An adapter's step through frozen layers, captured after a warm-up on a side stream and
+    replayed on new inputs."""
+    from ltx_kernels.blockwise import BlockwiseFP8FeedForward
+    low, lin = _lora(256, 256, 16, cuda_device, 121), _linear(256, 256, cuda_device, 124)
+    ff = BlockwiseFP8FeedForward.from_linears(_linear(512, 256, cuda_device, 126), _linear(256, 512, cuda_device, 128))
+    x = tokens(64, 256, 130).view(2, 32, 256).to(cuda_device)
+    dy = (grads(64, 256, 131) * 1e3).view(2, 32, 256).to(cuda_device)
+
+    def step():
+        return torch.autograd.grad(ff(lin(low(x))), (low.lora_A, low.lora_B), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    x.copy_(tokens(64, 256, 132).view(2, 32, 256))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
